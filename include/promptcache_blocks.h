@@ -860,6 +860,119 @@ int pcb_rec_prompt(const pcb_rec_args* a, void* stream);
 int32_t pcb_rec_step_fits(int32_t dim, int32_t vdim);
 int pcb_rec_step(const pcb_rec_args* a, void* stream);
 
+/* ---- keys and values in 8 bits, in pages -------------------------------------------------------------------------------------------
+ *
+ * A pool of n_pages pages of page_size tokens (P: 16, 32, 64 or 128) for each layer.  Of page p and key head h it holds
+ *   kcodes[p][h][t][d]   the keys' codes, row by row          vcodes[p][h][d][t]   the values' codes, column by column
+ *   kscale[p][h], vscale[p][h]   fp32: powers of two, exponents -40 .. 40;   a number is code * scale
+ * (d < dim; dim a multiple of 16 up to 256).  `code`: PCB_CODE_E4M3 (4 exponent bits, bias 7, 3 bits behind the point, largest 448) or
+ * PCB_CODE_INT8 (-127 .. 127).  The codes of columns are what attention's second product reads: a lane gets sixteen keys of a column in one load.
+ * Position i of sequence s is in page table[s][i / P], place i % P; its slot is that page's number * P + i % P.  Pages may be shared by several
+ * sequences as long as nobody appends to them.  All pools start on 16 bytes. */
+#define PCB_CODE_E4M3 0
+#define PCB_CODE_INT8 1
+
+/* A step's tables from its sequences' lengths, all on the device.  Sequence s holds cached[s] tokens and brings brings[s] (below zero: it is over).
+ *   have = ceil(cached / P), need = ceil((cached + brings) / P) - have; a sequence is GRANTED its tokens when they fit (need + have <= max_pages, its last
+ *   row below n_rows) and need is 0 or the sum of the needs up to and with its own is at most the free pages; one that is not granted keeps what it had
+ * ring (int32 [ring_cap]) holds the free pages: ring_state[0] the place of the first, ring_state[1] their number.  The granted sequences' pages are taken
+ * from its front, in order, and become table[s][have ..]; a sequence that is over gives its pages table[s][keep[s] .. have - 1] back at its end (keep null: 0;
+ * they are not handed out in the same call; its table is left as it is).  ring_out (int32 [4], may be ring_state) receives the new state {first, number, 0, 0};
+ * its third number is 0 before every call.  ring null: nothing is taken or given back, and the table already holds every page that is asked for.
+ * Results (optional but for row_slot; behind what there is, rows get -1 and tiles {-1, 0, 0, 0}):
+ *   kv_len [n_seqs]      tokens after the step: cached + brings, cached where not granted, 0 for one that is over (may be `cached`)
+ *   row_start [n_seqs + 1]   each sequence's first flat row, granted or not
+ *   row_seq, row_pos, row_slot (int64) [n_rows]   of every flat row; the slot is -1 where the sequence was not granted
+ *   tiles [n_tiles][4]   the granted sequences' rows in tiles {sequence, first position, rows (<= tile_rows), first flat row}; n_tiles >= n_seqs + n_rows / tile_rows
+ *   status [2]           sequences that were not granted, rows that were */
+typedef struct pcb_page_tables_args {
+    uint32_t struct_bytes;
+    int32_t n_seqs, max_pages;
+    int64_t ld_table;
+    int32_t page_size;
+    const int32_t* cached;
+    const int32_t* brings;
+    const int32_t* keep;
+    int32_t* table;
+    int32_t* ring;
+    int32_t ring_cap;
+    const int32_t* ring_state;
+    int32_t* ring_out;
+    int32_t* kv_len;
+    int32_t* row_start;
+    int32_t* row_seq;
+    int32_t* row_pos;
+    int64_t* row_slot;
+    int32_t n_rows;
+    int32_t* tiles;
+    int32_t n_tiles, tile_rows;
+    int32_t* status;
+} pcb_page_tables_args;
+int pcb_page_tables(const pcb_page_tables_args* a, void* stream);
+
+/* New rows into the pool, and rows of it back.  Row r of k and v (E, head h at r * ldk + h * k_head_stride, likewise v; 16-byte pieces) belongs to row_slot[r];
+ * rows whose slot is below zero or outside the pool are passed over.
+ *
+ * pcb_pages_append: neighbouring rows of one page go in together; m = the largest magnitude of a head's new elements in that page (numbers that are not
+ * finite left out), e = the smallest exponent with m <= C 2^e (C = 448 or 127), at least -40 and at most 40.  The page's scale becomes 2^e, or stays as it is
+ * where it is larger and the rows do not start the page; where it grows, the codes in front of the first new row are rounded anew.  code = x / scale to the
+ * nearest, ties to even; beyond C: C; what is not a number: 0.  What a page held behind its first new row is given up.  All rows of a page in a call are
+ * neighbours and their slots differ; nothing else writes that page meanwhile.
+ * pcb_pages_read: k[r], v[r] = code * scale. */
+typedef struct pcb_pages_rows_args {
+    uint32_t struct_bytes;
+    int32_t dtype, code;
+    void* k;
+    int64_t ldk, k_head_stride;
+    void* v;
+    int64_t ldv, v_head_stride;
+    const int64_t* row_slot;
+    int32_t n_rows;
+    void* kcodes;
+    float* kscale;
+    void* vcodes;
+    float* vscale;
+    int32_t n_pages, page_size, Hkv, dim;
+} pcb_pages_rows_args;
+int pcb_pages_append(const pcb_pages_rows_args* a, void* stream);
+int pcb_pages_read(const pcb_pages_rows_args* a, void* stream);
+
+/* Causal softmax attention over such a pool.  Queries are flat rows (E, head h of row r at r * ldq + h * q_head_stride, out likewise; 16-byte pieces); tile t =
+ * {sequence, first position, query rows (<= tile_rows), first flat row}, the granted tiles of pcb_page_tables.  The query at position i sees key j of its
+ * sequence iff j <= i, j < kv_len[sequence], window <= 0 or i - j < window, and table[sequence][j / P] is a page of the pool.
+ *   out = sum_j e^(scale q.k_j) v_j / (sum_j e^(scale q.k_j) + e^sink[h]),   sink (fp32 [H]) optional; a row that sees nothing: 0
+ * Query head h reads key head h / (H / Hkv).  scale > 0.  Tiles without rows or of no sequence, and rows outside [0, n_rows), are passed over.
+ * longest: an upper bound of kv_len that the host knows (0: max_pages * P, which pcb_attn_pages_part is then given); it decides the number of key runs that workgroups of their own take, whose
+ * results need part: pcb_attn_pages_part(...) floats, aligned to 16 bytes; launches that may run at the same time need a part of their own. */
+typedef struct pcb_attn_pages_args {
+    uint32_t struct_bytes;
+    int32_t dtype, code;
+    const void* q;
+    int64_t ldq, q_head_stride;
+    const int32_t* tiles;
+    int32_t n_tiles, tile_rows, n_rows;
+    const int32_t* kv_len;
+    const int32_t* table;
+    int64_t ld_table;
+    int32_t n_seqs, max_pages;
+    const void* kcodes;
+    const float* kscale;
+    const void* vcodes;
+    const float* vscale;
+    int32_t n_pages, page_size;
+    int32_t H, Hkv, dim;
+    float scale;
+    int32_t window;
+    const float* sink;
+    void* out;
+    int64_t ldo, out_head_stride;
+    int32_t longest;
+    float* part;
+    int64_t part_floats;
+} pcb_attn_pages_args;
+int64_t pcb_attn_pages_part(int32_t n_rows, int32_t H, int32_t Hkv, int32_t dim, int32_t n_tiles, int32_t tile_rows, int32_t longest);
+int pcb_attn_pages(const pcb_attn_pages_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

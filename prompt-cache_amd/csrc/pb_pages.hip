@@ -1,0 +1,476 @@
+// The paged 8-bit cache beside its attention: a step's tables (pcb_page_tables), rows into pages and back (pcb_pages_append, pcb_pages_read).
+//
+// pcb_page_tables: every workgroup scans all sequences (a thread a sequence, in chunks of the workgroup) and knows each chunk's prefix sums; the flat rows,
+// tiles and pages of a chunk are then shared out among the workgroups, each found by a search in the chunk's sums in LDS.  A step's tables are bound by the
+// latency of the loads and of three scans one after the other, so a batch of one chunk and few rows is one workgroup.
+//
+// pcb_pages_append / pcb_pages_read: a wave takes the rows of one page (16 keys of it when reading) of one head, keys or values, by itself: no LDS, no barrier, and
+// the maximum of a page is a wave's reduction.  Both are bound by memory: rows in and codes out, each once.
+#include "pb_pages.h"
+
+namespace {
+using namespace pcb;
+
+// ---- tables -------------------------------------------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const T u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+// inclusive sums over the workgroup's threads; `all`: the whole sum
+template <int NT, typename T>
+__device__ __forceinline__ T block_scan(T v, T* part, int tid, T& all) {
+    const int lane = tid & 63, wave = tid >> 6;
+    v = wave_scan(v, lane);
+    __syncthreads();
+    if (lane == 63) part[wave] = v;
+    __syncthreads();
+    T before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+        if (w < wave) before += part[w];
+        all += part[w];
+    }
+    return before + v;
+}
+// the first thread whose sum is above x
+template <int NT>
+__device__ __forceinline__ int find(const int* sums, int x) {
+    int lo = 0, hi = NT - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (sums[mid] > x)
+            hi = mid;
+        else
+            lo = mid + 1;
+    }
+    return lo;
+}
+__device__ __forceinline__ int ring_at(int64_t i, int cap) { return (int)(i % cap); }
+
+template <int NT>
+__global__ __launch_bounds__(NT) void page_tables_kernel(pcb_page_tables_args a, int ps) {
+    __shared__ int64_t part64[NT / 64];
+    __shared__ int part[NT / 64];
+    __shared__ int stop_s[NT], take_s[NT], back_s[NT], tile_s[NT];    // inclusive sums over the chunk: rows, pages taken, pages given back, tiles
+    __shared__ int cached_s[NT], have_s[NT], keep_s[NT], count_s[NT]; // count: rows of a granted sequence, -1 where not granted
+    __shared__ int last;
+    const int tid = threadIdx.x, P = 1 << ps, gsz = gridDim.x, wg = blockIdx.x;
+    const int cap = a.ring ? a.ring_cap : 1;
+    int head = a.ring ? a.ring_state[0] % cap : 0, free_pages = a.ring ? a.ring_state[1] : 0;
+    head = head < 0 ? head + cap : head;                              // (a state that no call wrote stays inside the ring all the same)
+    free_pages = free_pages < 0 ? 0 : free_pages > cap ? cap : free_pages;
+    int64_t rows0 = 0;                                                // totals of the chunks before this one
+    int need0 = 0, take0 = 0, back0 = 0, tile0 = 0, refused = 0, given = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += NT) {
+        const int s = s0 + tid;
+        const bool live = s < a.n_seqs;
+        const int cached = live && a.cached[s] > 0 ? a.cached[s] : 0;
+        const int brings = live ? a.brings[s] : 0;
+        const bool over = brings < 0;
+        const int count = over ? 0 : brings;
+        const int have = (int)(((int64_t)cached + P - 1) >> ps);
+        const int64_t total = ((int64_t)cached + count + P - 1) >> ps;
+        int64_t rows_all;
+        const int64_t stop = rows0 + block_scan<NT>((int64_t)count, part64, tid, rows_all);
+        const bool fits = total <= a.max_pages && stop <= a.n_rows;
+        const int need = a.ring && live && !over && fits ? (int)total - have : 0;
+        int need_all;
+        const int upto = need0 + block_scan<NT>(need, part, tid, need_all);
+        const bool granted = live && !over && fits && (need == 0 || upto <= free_pages);
+        int keep = over && a.keep ? a.keep[s] : 0;
+        keep = keep < 0 ? 0 : keep;
+        const int back = a.ring && over && have <= a.max_pages && have > keep ? have - keep : 0;
+        const int tiles = granted ? (int)(((int64_t)count + a.tile_rows - 1) / a.tile_rows) : 0;
+        int take_all, back_all, tile_all;
+        take_s[tid] = block_scan<NT>(granted ? need : 0, part, tid, take_all);
+        back_s[tid] = block_scan<NT>(back, part, tid, back_all);
+        tile_s[tid] = block_scan<NT>(tiles, part, tid, tile_all);
+        stop_s[tid] = (int)(stop - rows0 > a.n_rows ? (int64_t)a.n_rows + 1 : stop - rows0);   // (rows behind n_rows are nobody's)
+        cached_s[tid] = cached, have_s[tid] = have, keep_s[tid] = keep, count_s[tid] = granted ? count : -1;
+        if (wg == 0) {
+            if (live) {
+                if (a.kv_len) a.kv_len[s] = over ? 0 : granted ? cached + count : cached;
+                if (a.row_start) {
+                    const int64_t first = stop - count;
+                    a.row_start[s] = (int)(first > 0x7fffffff ? 0x7fffffff : first);
+                    if (s == a.n_seqs - 1) a.row_start[a.n_seqs] = (int)(stop > 0x7fffffff ? 0x7fffffff : stop);
+                }
+            }
+            if (a.status) {
+                int n;
+                block_scan<NT>(live && !over && !granted ? 1 : 0, part, tid, n);
+                refused += n;
+                block_scan<NT>(granted ? count : 0, part, tid, n);
+                given += n;
+            }
+        }
+        __syncthreads();
+        const int at0 = wg * NT + tid, step = gsz * NT;
+        // the granted sequences' new pages, and the places of those that come back
+        for (int i = at0; i < take_all; i += step) {
+            const int t = find<NT>(take_s, i), j = i - (t ? take_s[t - 1] : 0);
+            a.table[(int64_t)(s0 + t) * a.ld_table + have_s[t] + j] = a.ring[ring_at((int64_t)head + take0 + i, cap)];
+        }
+        for (int i = at0; i < back_all; i += step) {
+            const int t = find<NT>(back_s, i), j = i - (t ? back_s[t - 1] : 0);
+            a.ring[ring_at((int64_t)head + free_pages + back0 + i, cap)] = a.table[(int64_t)(s0 + t) * a.ld_table + keep_s[t] + j];
+        }
+        const int n_here = rows_all > a.n_rows ? a.n_rows : (int)rows_all;
+        for (int i = at0; i < n_here; i += step) {
+            const int64_t r = rows0 + i;
+            if (r >= a.n_rows) break;
+            const int t = find<NT>(stop_s, i), k = i - (t ? stop_s[t - 1] : 0);
+            const int64_t pos = (int64_t)cached_s[t] + k;
+            int64_t slot = -1;
+            if (count_s[t] >= 0) {
+                const int q = (int)(pos >> ps);
+                const int before = t ? take_s[t - 1] : 0;
+                const int page = a.ring && q >= have_s[t] ? a.ring[ring_at((int64_t)head + take0 + before + q - have_s[t], cap)]
+                                                          : a.table[(int64_t)(s0 + t) * a.ld_table + q];
+                if (page >= 0) slot = (int64_t)page * P + (pos & (P - 1));
+            }
+            if (a.row_seq) a.row_seq[r] = s0 + t;
+            if (a.row_pos) a.row_pos[r] = (int)(pos > 0x7fffffff ? 0x7fffffff : pos);
+            a.row_slot[r] = slot;
+        }
+        if (a.tiles)
+            for (int i = at0; i < tile_all; i += step) {
+                const int t = find<NT>(tile_s, i), off = (i - (t ? tile_s[t - 1] : 0)) * a.tile_rows;
+                const int left = count_s[t] - off;
+                int4 rec;
+                rec.x = s0 + t, rec.y = cached_s[t] + off, rec.z = left < a.tile_rows ? left : a.tile_rows;
+                rec.w = (int)(rows0 + (t ? stop_s[t - 1] : 0)) + off;
+                if (tile0 + i < a.n_tiles) reinterpret_cast<int4*>(a.tiles)[tile0 + i] = rec;
+            }
+        rows0 += rows_all, need0 += need_all, take0 += take_all, back0 += back_all, tile0 += tile_all;
+        __syncthreads();
+    }
+    for (int64_t r = rows0 + wg * NT + tid; r < a.n_rows; r += gsz * NT) {
+        if (a.row_seq) a.row_seq[r] = -1;
+        if (a.row_pos) a.row_pos[r] = -1;
+        a.row_slot[r] = -1;
+    }
+    if (a.tiles)
+        for (int64_t t = (int64_t)tile0 + wg * NT + tid; t < a.n_tiles; t += gsz * NT) reinterpret_cast<int4*>(a.tiles)[t] = int4{-1, 0, 0, 0};
+    if (wg == 0 && tid == 0 && a.status) a.status[0] = refused, a.status[1] = given;
+    if (!a.ring) return;
+    // ring_out may be ring_state: it is written by the workgroup that arrives last, when all have read it
+    __syncthreads();
+    if (tid == 0) {
+        last = gsz == 1 || atomicAdd(&a.ring_out[2], 1) == gsz - 1;
+        if (last) {
+            a.ring_out[0] = ring_at((int64_t)head + take0, cap);
+            a.ring_out[1] = free_pages - take0 + back0;
+            a.ring_out[2] = 0, a.ring_out[3] = 0;
+        }
+    }
+}
+
+// ---- rows into pages ------------------------------------------------------------------------------------------------------------------------
+// eight neighbouring elements as floats
+__device__ __forceinline__ void row8(const bf16_t* p, float (&o)[8]) {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[2 * e] = __uint_as_float(w[e] << 16), o[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+}
+__device__ __forceinline__ void row8(const float* p, float (&o)[8]) {
+    const f4 a = *reinterpret_cast<const f4*>(p), b = *reinterpret_cast<const f4*>(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = a[e], o[4 + e] = b[e];
+}
+__device__ __forceinline__ void put8(bf16_t* p, const float (&o)[8]) {
+    *reinterpret_cast<u32x4*>(p) = u32x4{bf16_pair(o[0], o[1]), bf16_pair(o[2], o[3]), bf16_pair(o[4], o[5]), bf16_pair(o[6], o[7])};
+}
+__device__ __forceinline__ void put8(float* p, const float (&o)[8]) {
+    *reinterpret_cast<f4*>(p) = f4{o[0], o[1], o[2], o[3]};
+    *reinterpret_cast<f4*>(p + 4) = f4{o[4], o[5], o[6], o[7]};
+}
+__device__ __forceinline__ float size_of(float x) { return __builtin_fabsf(x) < __builtin_inff() ? __builtin_fabsf(x) : 0.0f; }
+
+// four codes anew, in units that are 1 / ratio times as large
+template <int CODE>
+__device__ __forceinline__ uint32_t again(uint32_t w, float ratio) {
+    float o[4];
+    from_codes<CODE>(w, o);
+    return to_codes<CODE>(o[0] * ratio, o[1] * ratio, o[2] * ratio, o[3] * ratio);
+}
+
+struct RowsView {
+    const int64_t* slot;
+    int n_rows, ps;
+    int64_t slots;                                                    // of the whole pool
+    __device__ __forceinline__ int64_t at(int64_t r) const {
+        if (r < 0 || r >= n_rows) return -1;
+        const int64_t s = slot[r];
+        return s >= 0 && s < slots ? s : -1;
+    }
+};
+
+// One wave: the rows r0 .. r0 + n - 1 (n <= P), all of one page, their first slot s0; `even`: their slots follow one another.
+template <typename E, int CODE, bool VALUES>
+__device__ void append_run(const pcb_pages_rows_args& a, const RowsView& v, int64_t r0, int n, int64_t s0, int off_min, bool even, int h, int lane) {
+    const int P = 1 << v.ps, dim = a.dim, cpr = dim / 8;
+    const int64_t page = s0 >> v.ps;
+    const E* src = (const E*)(VALUES ? a.v : a.k) + (int64_t)h * (VALUES ? a.v_head_stride : a.k_head_stride);
+    const int64_t ld = VALUES ? a.ldv : a.ldk;
+    float* scale = (VALUES ? a.vscale : a.kscale) + page * a.Hkv + h;
+    uint8_t* codes = (uint8_t*)(VALUES ? a.vcodes : a.kcodes) + (page * a.Hkv + h) * (int64_t)P * dim;
+    const int chunks = n * cpr;
+    float m = 0.0f;
+#pragma unroll 4
+    for (int i = lane; i < chunks; i += 64) {
+        const int r = i / cpr, c = i - r * cpr;
+        float x[8];
+        row8(src + (r0 + r) * ld + c * 8, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, size_of(x[e]));
+    }
+    float s = scale_for<CODE>(wave_max(m));
+    if (off_min > 0) {
+        const float old = *scale;
+        if (old >= s) {
+            s = old;
+        } else {
+            // the codes in front of the first new row, in the new units.  (An old scale of a page that this library wrote is a power of two.)
+            const float ratio = old * inv_pow2(s);
+            if (!VALUES) {
+                uint32_t* w = (uint32_t*)codes;
+                for (int i = lane; i < off_min * dim / 4; i += 64) w[i] = again<CODE>(w[i], ratio);
+            } else {
+                const int words = (off_min + 3) / 4;
+                for (int i = lane; i < words * dim; i += 64) {
+                    const int d = i / words, k = i - d * words;
+                    uint32_t* w = (uint32_t*)(codes + (int64_t)d * P) + k;
+                    const uint32_t was = *w, now = again<CODE>(was, ratio);
+                    const int left = off_min - 4 * k;                 // bytes of the word that are in front of the first new row
+                    const uint32_t keep = left >= 4 ? 0u : 0xffffffffu << (8 * left);
+                    *w = (now & ~keep) | (was & keep);
+                }
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (other lanes write the rest of these words)
+            }
+        }
+    }
+    if (lane == 0) *scale = s;
+    const float inv = inv_pow2(s);
+    if (!VALUES) {
+#pragma unroll 4
+        for (int i = lane; i < chunks; i += 64) {
+            const int r = i / cpr, c = i - r * cpr;
+            const int off = even ? (int)(s0 & (P - 1)) + r : (int)(v.at(r0 + r) & (P - 1));
+            float x[8];
+            row8(src + (r0 + r) * ld + c * 8, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= inv;
+            *reinterpret_cast<u32x2*>(codes + (int64_t)off * dim + c * 8) =
+                u32x2{to_codes<CODE>(x[0], x[1], x[2], x[3]), to_codes<CODE>(x[4], x[5], x[6], x[7])};
+        }
+        return;
+    }
+    // values: a lane takes a column; sixteen rows that fill a 16-byte piece of it go out at once
+    const int off0 = (int)(s0 & (P - 1));
+    for (int d0 = 0; d0 < dim; d0 += 64) {
+        const int d = d0 + lane;
+        if (d >= dim) break;
+        uint8_t* col = codes + (int64_t)d * P;
+        int r = 0;
+        while (r < n) {
+            if (even && (off0 + r) % 16 == 0 && n - r >= 16) {
+                float x[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = to_f32(src[(r0 + r + e) * ld + d]) * inv;
+                u32x4 w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = to_codes<CODE>(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+                *reinterpret_cast<u32x4*>(col + off0 + r) = w;
+                r += 16;
+            } else {
+                const int off = even ? off0 + r : (int)(v.at(r0 + r) & (P - 1));
+                col[off] = (uint8_t)(to_codes<CODE>(to_f32(src[(r0 + r) * ld + d]) * inv, 0.f, 0.f, 0.f) & 255u);
+                ++r;
+            }
+        }
+    }
+}
+
+// blockIdx.y: keys or values.  A wave looks at WIN rows of one head and takes the runs that start there.
+template <typename E, int CODE>
+__global__ __launch_bounds__(256) void pages_append_kernel(pcb_pages_rows_args a, RowsView v, int win) {
+    const int lane = threadIdx.x & 63;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int h = (int)(unit % a.Hkv);
+    const int64_t w0 = unit / a.Hkv * win;
+    if (w0 >= a.n_rows) return;
+    const int P = 1 << v.ps;
+    const int64_t mine = lane < win ? v.at(w0 + lane) : -1;
+    const int64_t prev = lane < win ? v.at(w0 + lane - 1) : -1;
+    uint64_t starts = __ballot(mine >= 0 && (prev < 0 || prev >> v.ps != mine >> v.ps));
+    while (starts) {
+        const int i = __builtin_ctzll(starts);
+        starts &= starts - 1;
+        const int64_t r0 = w0 + i, s0 = __shfl(mine, i, 64), page = s0 >> v.ps;
+        // how far the run goes, its smallest place and whether its slots follow one another (P <= 128: two looks)
+        int n = 0, off_min = P;
+        bool even = true, open = true;
+        for (int part = 0; part < P && open; part += 64) {
+            const int64_t s = part + lane < P ? v.at(r0 + part + lane) : -1;
+            const uint64_t in = __ballot(s >= 0 && s >> v.ps == page);
+            const int k = ~in ? __builtin_ctzll(~in) : 64;
+            open = k == 64;
+            n += k;
+            int o = lane < k ? (int)(s & (P - 1)) : P;
+#pragma unroll
+            for (int x = 32; x > 0; x >>= 1) o = min(o, __shfl_xor(o, x, 64));
+            off_min = min(off_min, o);
+            if (__ballot(lane < k && s != s0 + part + lane)) even = false;
+        }
+        if (blockIdx.y == 0)
+            append_run<E, CODE, false>(a, v, r0, n, s0, off_min, even, h, lane);
+        else
+            append_run<E, CODE, true>(a, v, r0, n, s0, off_min, even, h, lane);
+    }
+}
+
+// ---- rows out of pages ------------------------------------------------------------------------------------------------------------------------
+// A wave takes, of one head, the groups of rows that start in its window: neighbours whose slots follow one another within 16 slots from a multiple of 16.
+template <typename E, int CODE>
+__global__ __launch_bounds__(256) void pages_read_kernel(pcb_pages_rows_args a, RowsView v) {
+    constexpr int WIN = 16;
+    const int lane = threadIdx.x & 63, dim = a.dim, P = 1 << v.ps;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int h = (int)(unit % a.Hkv);
+    const int64_t w0 = unit / a.Hkv * WIN;
+    if (w0 >= a.n_rows) return;
+    if (blockIdx.y == 0) {
+        const int cpr = dim / 16;
+        for (int i = lane; i < WIN * cpr; i += 64) {
+            const int r = i / cpr, c = i - r * cpr;
+            const int64_t s = v.at(w0 + r);
+            if (s < 0) continue;
+            const int64_t page = s >> v.ps;
+            const u32x4 w = *reinterpret_cast<const u32x4*>((const uint8_t*)a.kcodes + ((page * a.Hkv + h) * P + (s & (P - 1))) * dim + c * 16);
+            const float sc = a.kscale[page * a.Hkv + h];
+            E* dst = (E*)a.k + (w0 + r) * a.ldk + (int64_t)h * a.k_head_stride + c * 16;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float o[8];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x[4];
+                    from_codes<CODE>(w[2 * half + e], x);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[4 * e + j] = x[j] * sc;
+                }
+                put8(dst + 8 * half, o);
+            }
+        }
+        return;
+    }
+    const int64_t mine = lane < WIN ? v.at(w0 + lane) : -1, prev = lane < WIN ? v.at(w0 + lane - 1) : -1;
+    uint64_t starts = __ballot(mine >= 0 && (prev < 0 || prev + 1 != mine || mine % 16 == 0));
+    while (starts) {
+        const int i = __builtin_ctzll(starts);
+        starts &= starts - 1;
+        const int64_t r0 = w0 + i, s0 = __shfl(mine, i, 64), page = s0 >> v.ps;
+        const int most = 16 - (int)(s0 & 15);
+        const int64_t s = lane < most ? v.at(r0 + lane) : -1;
+        const uint64_t in = __ballot(s >= 0 && s == s0 + lane);
+        const int n = ~in ? __builtin_ctzll(~in) : 64;
+        const float sc = a.vscale[page * a.Hkv + h];
+        const uint8_t* codes = (const uint8_t*)a.vcodes + (page * a.Hkv + h) * (int64_t)P * dim + (s0 & (P - 1) & ~15);
+        E* dst = (E*)a.v + r0 * a.ldv + (int64_t)h * a.v_head_stride;
+        const int first = (int)(s0 & 15);
+        for (int d = lane; d < dim; d += 64) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(codes + (int64_t)d * P);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float x[4];
+                from_codes<CODE>(w[e], x);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int k = 4 * e + j - first;
+                    if (k >= 0 && k < n) dst[k * a.ldv + d] = from_f32<E>(x[j] * sc);
+                }
+            }
+        }
+    }
+}
+
+int check_rows(const pcb_pages_rows_args* a, const char* who) {
+    PCB_REQUIRE(a && a->struct_bytes == sizeof(pcb_pages_rows_args), PCB_ERR_ARG, "%s: struct size mismatch", who);
+    PCB_REQUIRE((a->dtype == PCB_BF16 || a->dtype == PCB_F32) && (a->code == PCB_CODE_E4M3 || a->code == PCB_CODE_INT8), PCB_ERR_ARG, "%s: unknown dtype or code", who);
+    PCB_REQUIRE(a->n_rows >= 0 && a->n_pages > 0 && pcb_page_size_ok(a->page_size) && a->Hkv > 0 && a->dim > 0 && a->dim <= 256 && a->dim % 16 == 0, PCB_ERR_ARG,
+                "%s: bad sizes (pages of 16, 32, 64 or 128 tokens, heads of a multiple of 16 up to 256)", who);
+    if (a->n_rows == 0) return PCB_OK;
+    const int es = a->dtype == PCB_BF16 ? 8 : 4;
+    PCB_REQUIRE(a->k && a->v && a->row_slot && a->kcodes && a->kscale && a->vcodes && a->vscale, PCB_ERR_ARG, "%s: null pointer", who);
+    PCB_REQUIRE(((uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->kcodes | (uintptr_t)a->vcodes) % 16 == 0 && (uintptr_t)a->row_slot % 8 == 0 && a->ldk % es == 0 &&
+                    a->ldv % es == 0 && a->k_head_stride % es == 0 && a->v_head_stride % es == 0,
+                PCB_ERR_ARG, "%s: rows, heads and codes start on 16 bytes", who);
+    PCB_REQUIRE(((int64_t)a->n_rows + 15) / 16 * a->Hkv <= (int64_t)1 << 25, PCB_ERR_ARG, "%s: too many rows (n_rows * Hkv up to 2^29)", who);
+    return PCB_OK;
+}
+
+}  // namespace
+
+PCB_EXPORT int pcb_page_tables(const pcb_page_tables_args* a, void* stream) {
+    PCB_REQUIRE(a && a->struct_bytes == sizeof(pcb_page_tables_args), PCB_ERR_ARG, "pcb_page_tables: struct size mismatch");
+    PCB_REQUIRE(a->n_seqs > 0 && a->max_pages > 0 && a->ld_table >= a->max_pages && pcb_page_size_ok(a->page_size) && a->n_rows >= 0 && (int64_t)a->n_seqs * a->max_pages < 0x7fffffff &&
+                    (int64_t)a->max_pages * a->page_size <= 0x7fffffff,
+                PCB_ERR_ARG, "pcb_page_tables: bad sizes (pages of 16, 32, 64 or 128 tokens, positions of 31 bits)");
+    PCB_REQUIRE(a->cached && a->brings && a->table && (a->row_slot || a->n_rows == 0), PCB_ERR_ARG, "pcb_page_tables: null pointer");
+    PCB_REQUIRE(!a->ring || (a->ring_cap > 0 && a->ring_state && a->ring_out), PCB_ERR_ARG, "pcb_page_tables: a ring comes with its state, and a place for the new one");
+    PCB_REQUIRE(!a->tiles || (a->tile_rows > 0 && (uintptr_t)a->tiles % 16 == 0 && a->n_tiles >= (int64_t)a->n_seqs + a->n_rows / a->tile_rows), PCB_ERR_ARG,
+                "pcb_page_tables: tiles on 16 bytes, n_seqs + n_rows / tile_rows of them");
+    pcb_page_tables_args b = *a;
+    if (!b.tiles) b.tile_rows = 1, b.n_tiles = 0;
+    // one workgroup while a chunk holds all sequences and four trips all rows; never more where kv_len is `cached`, which the others still read.
+    const bool one = a->kv_len == a->cached || (a->n_seqs <= 1024 && a->n_rows <= 4096);
+    int groups = one ? 1 : pcb_ceil_div(a->n_rows > a->n_seqs ? a->n_rows : a->n_seqs, 1024);
+    if (groups > 128) groups = 128;
+    if (groups < 1) groups = 1;
+    const int ps = pcb_log2(a->page_size);
+    if (a->n_seqs <= 256 && a->n_rows <= 1024)
+        hipLaunchKernelGGL(page_tables_kernel<256>, dim3(groups), dim3(256), 0, (hipStream_t)stream, b, ps);
+    else
+        hipLaunchKernelGGL(page_tables_kernel<1024>, dim3(groups), dim3(1024), 0, (hipStream_t)stream, b, ps);
+    return pcb_check_launch("page_tables_kernel");
+}
+
+#define PCB_PAGES_LAUNCH(KERNEL, GRID, ...)                                                                                      \
+    do {                                                                                                                         \
+        if (a->dtype == PCB_BF16 && a->code == PCB_CODE_E4M3)                                                                    \
+            hipLaunchKernelGGL((KERNEL<pcb::bf16_t, PCB_CODE_E4M3>), GRID, dim3(256), 0, (hipStream_t)stream, *a, __VA_ARGS__);  \
+        else if (a->dtype == PCB_BF16)                                                                                           \
+            hipLaunchKernelGGL((KERNEL<pcb::bf16_t, PCB_CODE_INT8>), GRID, dim3(256), 0, (hipStream_t)stream, *a, __VA_ARGS__);  \
+        else if (a->code == PCB_CODE_E4M3)                                                                                       \
+            hipLaunchKernelGGL((KERNEL<float, PCB_CODE_E4M3>), GRID, dim3(256), 0, (hipStream_t)stream, *a, __VA_ARGS__);        \
+        else                                                                                                                     \
+            hipLaunchKernelGGL((KERNEL<float, PCB_CODE_INT8>), GRID, dim3(256), 0, (hipStream_t)stream, *a, __VA_ARGS__);        \
+    } while (0)
+
+PCB_EXPORT int pcb_pages_append(const pcb_pages_rows_args* a, void* stream) {
+    const int rc = check_rows(a, "pcb_pages_append");
+    if (rc != PCB_OK || a->n_rows == 0) return rc;
+    const RowsView v{a->row_slot, a->n_rows, pcb_log2(a->page_size), (int64_t)a->n_pages * a->page_size};
+    const int win = (int64_t)a->n_rows * a->Hkv <= 16384 ? 1 : 16;      // rows of different requests side by side; or prompts, whose windows start at most a page or two
+    const int64_t waves = ((int64_t)a->n_rows + win - 1) / win * a->Hkv;
+    const dim3 grid((unsigned)((waves + 3) / 4), 2);
+    PCB_PAGES_LAUNCH(pages_append_kernel, grid, v, win);
+    return pcb_check_launch("pages_append_kernel");
+}
+
+PCB_EXPORT int pcb_pages_read(const pcb_pages_rows_args* a, void* stream) {
+    const int rc = check_rows(a, "pcb_pages_read");
+    if (rc != PCB_OK || a->n_rows == 0) return rc;
+    const RowsView v{a->row_slot, a->n_rows, pcb_log2(a->page_size), (int64_t)a->n_pages * a->page_size};
+    const int64_t waves = ((int64_t)a->n_rows + 15) / 16 * a->Hkv;
+    const dim3 grid((unsigned)((waves + 3) / 4), 2);
+    PCB_PAGES_LAUNCH(pages_read_kernel, grid, v);
+    return pcb_check_launch("pages_read_kernel");
+}

@@ -20,6 +20,8 @@ ACT_NONE, ACT_SILU, ACT_SIGMOID, ACT_RELU2, ACT_SOFTPLUS, ACT_SOFTCAP, ACT_RELU,
 NOT_TAKEN, NORM_LINEAR_MAX = 1, 16384                              # (what norm_linear takes: rows x columns)
 NORM_NONE, NORM_RMS, NORM_DYT = 0, 1, 2
 SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1
+CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}                    # of paged keys and values
+PAGE_SIZES = (16, 32, 64, 128)
 ABI_VERSION = 6
 DTYPES = {torch.bfloat16: BF16, torch.float32: F32}
 
@@ -208,6 +210,32 @@ class RecArgs(C.Structure):
                 ("gain", _vp), ("eps", _f32), ("gate", _vp), ("ldg", _i64), ("y", _vp), ("ldy", _i64)]
 
 
+class PageTablesArgs(C.Structure):
+    """``pcb_page_tables_args`` (field for field)."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("n_seqs", _i32), ("max_pages", _i32), ("ld_table", _i64), ("page_size", _i32),
+                ("cached", _vp), ("brings", _vp), ("keep", _vp), ("table", _vp), ("ring", _vp), ("ring_cap", _i32), ("ring_state", _vp), ("ring_out", _vp),
+                ("kv_len", _vp), ("row_start", _vp), ("row_seq", _vp), ("row_pos", _vp), ("row_slot", _vp), ("n_rows", _i32),
+                ("tiles", _vp), ("n_tiles", _i32), ("tile_rows", _i32), ("status", _vp)]
+
+
+class PagesRowsArgs(C.Structure):
+    """``pcb_pages_rows_args`` (field for field)."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("dtype", _i32), ("code", _i32),
+                ("k", _vp), ("ldk", _i64), ("k_head_stride", _i64), ("v", _vp), ("ldv", _i64), ("v_head_stride", _i64),
+                ("row_slot", _vp), ("n_rows", _i32), ("kcodes", _vp), ("kscale", _vp), ("vcodes", _vp), ("vscale", _vp),
+                ("n_pages", _i32), ("page_size", _i32), ("Hkv", _i32), ("dim", _i32)]
+
+
+class AttnPagesArgs(C.Structure):
+    """``pcb_attn_pages_args`` (field for field)."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("dtype", _i32), ("code", _i32),
+                ("q", _vp), ("ldq", _i64), ("q_head_stride", _i64), ("tiles", _vp), ("n_tiles", _i32), ("tile_rows", _i32), ("n_rows", _i32),
+                ("kv_len", _vp), ("table", _vp), ("ld_table", _i64), ("n_seqs", _i32), ("max_pages", _i32),
+                ("kcodes", _vp), ("kscale", _vp), ("vcodes", _vp), ("vscale", _vp), ("n_pages", _i32), ("page_size", _i32),
+                ("H", _i32), ("Hkv", _i32), ("dim", _i32), ("scale", _f32), ("window", _i32), ("sink", _vp),
+                ("out", _vp), ("ldo", _i64), ("out_head_stride", _i64), ("longest", _i32), ("part", _vp), ("part_floats", _i64)]
+
+
 # name -> (restype, argtypes); mirrors include/promptcache_blocks.h one to one
 SIGNATURES = {
     "pcb_version": (C.c_int, []),
@@ -263,6 +291,11 @@ SIGNATURES = {
     "pcb_rec_prompt": (C.c_int, [C.POINTER(RecArgs), _vp]),
     "pcb_rec_step_fits": (C.c_int32, [_i32, _i32]),
     "pcb_rec_step": (C.c_int, [C.POINTER(RecArgs), _vp]),
+    "pcb_page_tables": (C.c_int, [C.POINTER(PageTablesArgs), _vp]),
+    "pcb_pages_append": (C.c_int, [C.POINTER(PagesRowsArgs), _vp]),
+    "pcb_pages_read": (C.c_int, [C.POINTER(PagesRowsArgs), _vp]),
+    "pcb_attn_pages_part": (_i64, [_i32] * 7),
+    "pcb_attn_pages": (C.c_int, [C.POINTER(AttnPagesArgs), _vp]),
 }
 
 
@@ -1148,3 +1181,115 @@ def rec_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lds_, reqs: torc
     a = _rec_args(q, k, v, lds_, reqs, n_reqs, state, H, Hk, dim, vdim, **kw)
     a.gain, a.eps, a.gate, a.ldg, a.y, a.ldy = _p(gain), float(eps), _p(gate), ldg, _p(y), ldy
     check(load().pcb_rec_step(C.byref(a), _stream()), "pcb_rec_step")
+
+
+# ---- keys and values in 8 bits, in pages ------------------------------------------------------------------------------------------------------
+def _flat(t: Optional[torch.Tensor], dtype, numel: int, what: str) -> None:
+    """``t`` (optional) holds at least ``numel`` elements of ``dtype`` one after the other on the current device."""
+    if t is None:
+        return
+    _want(t, dtype, what)
+    if t.numel() < numel:
+        raise ValueError(f"{what}: {numel} elements are needed, got {t.numel()}")
+    _here(t, what)
+
+
+def _here(t: torch.Tensor, what: str) -> None:
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what} lies on {t.device}, and the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _pool(kcodes: torch.Tensor, kscale: torch.Tensor, vcodes: torch.Tensor, vscale: torch.Tensor, what: str):
+    """Checks a pool: codes ``[pages, Hkv, P, dim]`` / ``[pages, Hkv, dim, P]``, scales ``[pages, Hkv]``; -> (code, pages, P, Hkv, dim)."""
+    if kcodes.dtype not in CODES or vcodes.dtype != kcodes.dtype:
+        raise TypeError(f"{what}: codes are both float8_e4m3fn or both int8, got {kcodes.dtype} and {vcodes.dtype}")
+    if kcodes.dim() != 4 or vcodes.shape != (kcodes.shape[0], kcodes.shape[1], kcodes.shape[3], kcodes.shape[2]):
+        raise ValueError(f"{what}: key codes [pages, heads, P, dim] and value codes [pages, heads, dim, P], got {tuple(kcodes.shape)} and {tuple(vcodes.shape)}")
+    pages, Hkv, P, dim = kcodes.shape
+    _flat(kcodes, kcodes.dtype, 0, f"{what} key codes"); _flat(vcodes, kcodes.dtype, 0, f"{what} value codes")
+    _flat(kscale, torch.float32, pages * Hkv, f"{what} key scales"); _flat(vscale, torch.float32, pages * Hkv, f"{what} value scales")
+    return CODES[kcodes.dtype], pages, P, Hkv, dim
+
+
+def _heads(t: torch.Tensor, heads: int, dim: int, what: str):
+    """Rows ``[rows, heads, dim]`` with neighbouring elements of a head; -> (row stride, head stride)."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or (t.stride(2) != 1 and t.numel() > 0):
+        raise ValueError(f"{what}: rows [rows, {heads}, {dim}] whose last axis is contiguous, got {tuple(t.shape)} with strides {t.stride()}")
+    _here(t, what)
+    return t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if heads > 1 else 0
+
+
+def page_tables(cached: torch.Tensor, brings: torch.Tensor, table: torch.Tensor, page_size: int, *, row_slot: torch.Tensor, kv_len=None, row_start=None, row_seq=None,
+                row_pos=None, tiles=None, tile_rows: int = 1, status=None, ring=None, ring_state=None, ring_out=None, keep=None) -> None:
+    """Block tables, slots and tiles of a step from its sequences' lengths, on the device.  ``cached`` / ``brings`` int32 [n]: tokens a sequence holds
+    and brings (below zero: it is over); ``table`` int32 [n, max_pages] gets the pages taken from ``ring`` (int32, the free pages; ``ring_state`` int32 [2 or
+    more] {first, number}; ``ring_out`` int32 [4], may be ``ring_state``).  ``row_slot`` int64 [rows] and, optional, ``row_seq`` / ``row_pos`` int32 [rows],
+    ``row_start`` [n + 1], ``kv_len`` [n], ``tiles`` [n + rows // tile_rows, 4], ``status`` [2] are written; without ``ring`` the table holds all pages already."""
+    n, rows = cached.numel(), row_slot.numel()
+    if table.dim() != 2 or table.shape[0] < n or table.dtype != torch.int32 or table.stride(1) != 1 or table.stride(0) < table.shape[1]:
+        raise ValueError(f"page_tables table: int32 [{n}, pages] with contiguous rows, got {table.dtype} {tuple(table.shape)}")
+    _here(table, "page_tables table")
+    for t, dtype, numel, what in ((cached, torch.int32, n, "cached"), (brings, torch.int32, n, "brings"), (keep, torch.int32, n, "keep"), (kv_len, torch.int32, n, "kv_len"),
+                                  (row_start, torch.int32, n + 1, "row_start"), (row_seq, torch.int32, rows, "row_seq"), (row_pos, torch.int32, rows, "row_pos"),
+                                  (row_slot, torch.int64, rows, "row_slot"), (status, torch.int32, 2, "status"), (ring, torch.int32, 1, "ring"),
+                                  (ring_state, torch.int32, 2, "ring_state"), (ring_out, torch.int32, 4, "ring_out"), (tiles, torch.int32, 0, "tiles")):
+        _flat(t, dtype, numel, "page_tables " + what)
+    a = PageTablesArgs(C.sizeof(PageTablesArgs), n, table.shape[1], table.stride(0), page_size, _p(cached), _p(brings), _p(keep), _p(table),
+                       _p(ring), 0 if ring is None else ring.numel(), _p(ring_state), _p(ring_out), _p(kv_len), _p(row_start), _p(row_seq), _p(row_pos), _p(row_slot), rows,
+                       _p(tiles), 0 if tiles is None else tiles.numel() // 4, tile_rows, _p(status))
+    check(load().pcb_page_tables(C.byref(a), _stream()), "pcb_page_tables")
+
+
+def _pages_rows(name: str, k, v, row_slot, kcodes, kscale, vcodes, vscale) -> None:
+    code, pages, P, Hkv, dim = _pool(kcodes, kscale, vcodes, vscale, name)
+    if k.dtype != v.dtype or k.shape != v.shape:
+        raise TypeError(f"{name}: keys and values of one type and shape, got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
+    _flat(row_slot, torch.int64, k.shape[0], f"{name} row_slot")
+    a = PagesRowsArgs(C.sizeof(PagesRowsArgs), _code(k), code, _p(k), *_heads(k, Hkv, dim, f"{name} keys"), _p(v), *_heads(v, Hkv, dim, f"{name} values"), _p(row_slot),
+                      k.shape[0], _p(kcodes), _p(kscale), _p(vcodes), _p(vscale), pages, P, Hkv, dim)
+    check(getattr(load(), "pcb_" + name)(C.byref(a), _stream()), "pcb_" + name)
+
+
+def pages_append(k: torch.Tensor, v: torch.Tensor, row_slot: torch.Tensor, kcodes: torch.Tensor, kscale: torch.Tensor, vcodes: torch.Tensor, vscale: torch.Tensor) -> None:
+    """Rows ``k`` / ``v`` [rows, Hkv, dim] into the pool at ``row_slot`` int64 [rows] (below zero: passed over); see ``pcb_pages_append`` for a page's scale.
+    All rows of a page are neighbours, and their slots differ."""
+    _pages_rows("pages_append", k, v, row_slot, kcodes, kscale, vcodes, vscale)
+
+
+def pages_read(row_slot: torch.Tensor, kcodes: torch.Tensor, kscale: torch.Tensor, vcodes: torch.Tensor, vscale: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+    """The pool's rows at ``row_slot`` as numbers into ``k`` / ``v`` [rows, Hkv, dim]; rows of a slot below zero are left as they are."""
+    _pages_rows("pages_read", k, v, row_slot, kcodes, kscale, vcodes, vscale)
+
+
+def attn_pages_part(rows: int, H: int, Hkv: int, dim: int, n_tiles: int, tile_rows: int, longest: int) -> int:
+    """Floats of the scratch that ``attn_pages`` needs for these sizes (0: none)."""
+    n = load().pcb_attn_pages_part(rows, H, Hkv, dim, n_tiles, tile_rows, longest)
+    if n < 0:
+        check(int(n), "pcb_attn_pages_part")
+    return int(n)
+
+
+def attn_pages(q: torch.Tensor, tiles: torch.Tensor, tile_rows: int, kv_len: torch.Tensor, table: torch.Tensor, kcodes: torch.Tensor, kscale: torch.Tensor,
+               vcodes: torch.Tensor, vscale: torch.Tensor, out: torch.Tensor, *, scale: float, window: int = 0, sink=None, longest: int = 0, part=None) -> None:
+    """Causal attention of rows ``q`` [rows, H, dim] over the pages of ``table`` int32 [n, max_pages], ``kv_len`` int32 [n] tokens of which are written; ``tiles`` int32
+    [t, 4] {sequence, first position, rows, first flat row} as ``page_tables`` makes them, of at most ``tile_rows`` rows; ``sink`` fp32 [H].  ``longest``: an upper bound
+    of ``kv_len`` known to the host (0: the table's width); ``part`` fp32 of ``attn_pages_part(...)`` floats (None: allocated when it is needed)."""
+    code, pages, P, Hkv, dim = _pool(kcodes, kscale, vcodes, vscale, "attn_pages")
+    if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype or q.shape[1] % Hkv:
+        raise ValueError(f"attn_pages: queries and results [rows, H, {dim}], H a multiple of {Hkv}, of one type; got {q.dtype} {tuple(q.shape)} and {out.dtype} {tuple(out.shape)}")
+    rows, H = q.shape[0], q.shape[1]
+    n = kv_len.numel()
+    if table.dim() != 2 or table.shape[0] < n or table.dtype != torch.int32 or table.stride(1) != 1:
+        raise ValueError(f"attn_pages table: int32 [{n}, pages] with contiguous rows, got {table.dtype} {tuple(table.shape)}")
+    _here(table, "attn_pages table")
+    _flat(tiles, torch.int32, 0, "attn_pages tiles"); _flat(kv_len, torch.int32, 0, "attn_pages kv_len")
+    _flat(sink, torch.float32, H, "attn_pages sink"); _flat(part, torch.float32, 0, "attn_pages part")
+    longest = longest if longest > 0 else table.shape[1] * P
+    n_tiles = tiles.numel() // 4
+    if part is None:
+        floats = attn_pages_part(rows, H, Hkv, dim, n_tiles, tile_rows, longest)
+        part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    a = AttnPagesArgs(C.sizeof(AttnPagesArgs), _code(q), code, _p(q), *_heads(q, H, dim, "attn_pages queries"), _p(tiles), n_tiles, tile_rows, rows, _p(kv_len), _p(table),
+                      table.stride(0), n, table.shape[1], _p(kcodes), _p(kscale), _p(vcodes), _p(vscale), pages, P, H, Hkv, dim, float(scale), int(window), _p(sink),
+                      _p(out), *_heads(out, H, dim, "attn_pages results"), longest, _p(part), 0 if part is None else part.numel())
+    check(load().pcb_attn_pages(C.byref(a), _stream()), "pcb_attn_pages")

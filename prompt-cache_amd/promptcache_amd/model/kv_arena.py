@@ -413,3 +413,132 @@ class SlotArena:
     def keys(self, layer: int, slot: int) -> torch.Tensor:
         """``[kv_heads, length, head_dim]`` view of one slot's keys."""
         return self.planes[layer][slot, :, :self.lengths[slot]]
+
+
+class PageStep:
+    """What a ``PageCache`` knows of one step, all on the device but ``rows``, ``tile_rows`` and ``longest``: ``row_slot`` (-1: the row has no place), ``row_seq``, ``row_pos``
+    per flat row, ``row_start`` per sequence, ``tiles`` of at most ``tile_rows`` rows, ``status`` {sequences refused, rows granted}, ``kv_len`` per sequence.  Its
+    buffers belong to the cache and hold until its next step."""
+
+    __slots__ = ("rows", "tile_rows", "longest", "row_slot", "row_seq", "row_pos", "row_start", "tiles", "status", "kv_len")
+
+
+class PageCache:
+    """Keys and values in 8 bits (``codes``: float8_e4m3fn or int8) in pages of ``page_size`` tokens, a power-of-two scale for each page and key head: half the bytes of a
+    16-bit ``SlotArena``, pages taken as sequences grow instead of rows of one capacity, and whole pages shared between sequences (``share``).
+
+    A step is ``begin`` (block tables, slots and tiles on the device, from the lengths that live there), then per layer ``append`` and ``attend``.  Nothing waits for
+    the device, so a step of one token a sequence can be captured into a graph and replayed: its tables move on by themselves.  Rows are flat, the sequences' new
+    tokens one after another; a sequence that finds no free page is refused as a whole (``status``), keeps what it had and gets no slots.
+
+    ``layer_dims``: (key heads, head size) per layer, sizes multiples of 16 up to 256; ``max_pages``: pages a sequence may have."""
+
+    def __init__(self, layer_dims, seqs: int, pages: int, device, *, page_size: int = 64, max_pages: Optional[int] = None, codes=torch.float8_e4m3fn):
+        from .. import _blocks as B
+        if codes not in B.CODES or page_size not in B.PAGE_SIZES:
+            raise ValueError(f"codes are float8_e4m3fn or int8 in pages of {B.PAGE_SIZES} tokens, got {codes} and {page_size}")
+        self.layer_dims = [(int(g), int(d)) for g, d in layer_dims]
+        if seqs < 1 or pages < 1 or any(g < 1 or d < 16 or d > 256 or d % 16 for g, d in self.layer_dims):
+            raise ValueError("at least one sequence and one page, heads of a multiple of 16 up to 256")
+        self.seqs, self.pages, self.page_size, self.codes, self.device = seqs, pages, page_size, codes, torch.device(device)
+        self.max_pages = pages if max_pages is None else max_pages
+        if self.max_pages < 1 or self.max_pages * page_size > 2 ** 31 - 128:
+            raise ValueError("a sequence has at least one page, and positions of 31 bits")
+        raw = [(torch.zeros((pages, g, page_size, d), dtype=torch.uint8, device=device), torch.zeros((pages, g, d, page_size), dtype=torch.uint8, device=device))
+               for g, d in self.layer_dims]
+        self.kcodes, self.vcodes = [k.view(codes) for k, _ in raw], [v.view(codes) for _, v in raw]
+        self.kscale = [torch.ones((pages, g), dtype=torch.float32, device=device) for g, _ in self.layer_dims]
+        self.vscale = [torch.ones((pages, g), dtype=torch.float32, device=device) for g, _ in self.layer_dims]
+        self.table = torch.full((seqs, self.max_pages), -1, dtype=torch.int32, device=device)
+        self.cached = torch.zeros(seqs, dtype=torch.int32, device=device)
+        self.keep = torch.zeros(seqs, dtype=torch.int32, device=device)
+        self.ring = torch.arange(pages, dtype=torch.int32, device=device)
+        self.ring_state = torch.tensor([0, pages, 0, 0], dtype=torch.int32, device=device)
+        self._bufs, self._outgrown, self._shared = {}, [], False
+
+    def bytes_per_token(self) -> float:
+        """Bytes that one token takes, its part of the scales with it."""
+        return sum(2 * g * (d + 4 / self.page_size) for g, d in self.layer_dims)
+
+    def _buf(self, name: str, shape, dtype) -> torch.Tensor:
+        """A named buffer's first elements as a tensor of this shape; it grows by doubling, and what it outgrew stays alive for launches that were captured with it."""
+        n = 1
+        for v in shape:
+            n *= v
+        t = self._bufs.get(name)
+        if t is None or t.numel() < n:
+            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a step's buffers are made by an eager run of the same sizes before a capture")
+            if t is not None:
+                self._outgrown.append(t)
+            t = self._bufs[name] = torch.zeros(max(n, 2 * t.numel() if t is not None else 0), dtype=dtype, device=self.device)
+        return t[:n].view(shape)
+
+    def begin(self, brings, rows: int, *, tile_rows: int = 1, longest: int = 0) -> PageStep:
+        """Tables of a step.  ``brings``: new tokens of every sequence (0: none, -1: the sequence is over and its pages are free), an int32 device tensor or numbers;
+        ``rows``: at least their sum (rows behind it have no slot); ``longest``: an upper bound of the lengths after the step, 0 where the host knows none."""
+        from .. import _blocks as B
+        if not isinstance(brings, torch.Tensor):
+            brings = uploaded(list(brings), torch.int32, self.device)
+        if brings.numel() != self.seqs or rows < 0 or tile_rows < 1:
+            raise ValueError(f"a step names the new tokens of all {self.seqs} sequences, its rows and tiles of at least one row")
+        s = PageStep()
+        s.rows, s.tile_rows, s.longest = rows, tile_rows, longest
+        s.row_slot, s.row_seq, s.row_pos = self._buf("slot", (rows,), torch.int64), self._buf("seq", (rows,), torch.int32), self._buf("pos", (rows,), torch.int32)
+        s.row_start, s.status = self._buf("start", (self.seqs + 1,), torch.int32), self._buf("status", (2,), torch.int32)
+        s.tiles = self._buf("tiles", (self.seqs + rows // tile_rows, 4), torch.int32)
+        B.page_tables(self.cached, brings, self.table, self.page_size, row_slot=s.row_slot, kv_len=self.cached, row_start=s.row_start, row_seq=s.row_seq, row_pos=s.row_pos,
+                      tiles=s.tiles, tile_rows=tile_rows, status=s.status, ring=self.ring, ring_state=self.ring_state, ring_out=self.ring_state, keep=self.keep)
+        if self._shared:
+            self.keep.masked_fill_(brings < 0, 0)                 # (whoever takes the sequence's place owns all of its pages)
+        s.kv_len = self.cached
+        return s
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, step: PageStep) -> None:
+        """The step's keys and values ``[rows, heads, dim]`` (bf16 or fp32) into their slots."""
+        from .. import _blocks as B
+        if k.shape[0] != step.rows:
+            raise ValueError(f"the step has {step.rows} rows, the keys {k.shape[0]}")
+        B.pages_append(k, v, step.row_slot, self.kcodes[layer], self.kscale[layer], self.vcodes[layer], self.vscale[layer])
+
+    def attend(self, layer: int, q: torch.Tensor, step: PageStep, *, scale: Optional[float] = None, window: int = 0, sink=None, out=None) -> torch.Tensor:
+        """Causal attention of the step's rows ``q`` [rows, H, dim] over everything their sequences hold, the step's own keys included (``append`` comes first); rows
+        without a slot are left as ``out`` has them (zeros where it is made here).  ``scale``: 1 / sqrt(dim) by default."""
+        from .. import _blocks as B
+        if q.shape[0] != step.rows:
+            raise ValueError(f"the step has {step.rows} rows, the queries {q.shape[0]}")
+        g, d = self.layer_dims[layer]
+        out = torch.zeros_like(q, memory_format=torch.contiguous_format) if out is None else out
+        longest = step.longest or self.max_pages * self.page_size
+        floats = B.attn_pages_part(step.rows, q.shape[1], g, d, step.tiles.shape[0], step.tile_rows, longest)
+        part = self._buf("part", (floats,), torch.float32) if floats else None
+        B.attn_pages(q, step.tiles, step.tile_rows, step.kv_len, self.table, self.kcodes[layer], self.kscale[layer], self.vcodes[layer], self.vscale[layer], out,
+                     scale=d ** -0.5 if scale is None else scale, window=window, sink=sink, longest=longest, part=part)
+        return out
+
+    def share(self, source: int, target: int, tokens: int) -> None:
+        """Sequence ``target`` starts with the first ``tokens`` tokens of ``source``, in the same pages: whole pages only, nobody appends to them.  ``target`` holds nothing
+        before; ``source`` stays until ``target`` is over (the pages are its own, and are free when it is over)."""
+        if tokens < 0 or tokens % self.page_size or tokens > self.max_pages * self.page_size or source == target or \
+                not (0 <= source < self.seqs and 0 <= target < self.seqs):
+            raise ValueError(f"sequences share whole pages of {self.page_size} tokens")
+        n = tokens // self.page_size
+        self.table[target, :n].copy_(self.table[source, :n])
+        self.cached[target:target + 1].fill_(tokens)
+        self.keep[target:target + 1].fill_(n)
+        self._shared = True
+
+    def read(self, layer: int, slots: torch.Tensor, dtype=torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values at ``slots`` (int64; -1: zeros) as dense rows ``[rows, heads, dim]``."""
+        from .. import _blocks as B
+        g, d = self.layer_dims[layer]
+        k, v = (torch.zeros((slots.numel(), g, d), dtype=dtype, device=self.device) for _ in range(2))
+        B.pages_read(slots, self.kcodes[layer], self.kscale[layer], self.vcodes[layer], self.vscale[layer], k, v)
+        return k, v
+
+    def rows(self, layer: int, seq: int, tokens: int, dtype=torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The first ``tokens`` tokens of a sequence as dense rows ``[tokens, heads, dim]``."""
+        from .. import _blocks as B
+        slots = torch.empty(tokens, dtype=torch.int64, device=self.device)
+        B.page_tables(torch.zeros(1, dtype=torch.int32, device=self.device), uploaded([tokens], torch.int32, self.device), self.table[seq:seq + 1], self.page_size, row_slot=slots)
+        return self.read(layer, slots, dtype)
