@@ -1,0 +1,79 @@
+// What the kernels behind pcb_attn_pages share: how a call is cut, tiles, results.
+#pragma once
+#include "pb_pages.h"
+
+#ifdef __HIPCC__
+namespace pcb {
+
+constexpr float LOG2E = 1.44269504088896f;
+constexpr float NEG = -__builtin_inff();
+
+constexpr int MANY_COLS = 128;
+constexpr int MAX_GROUPS = 512;        // workgroups that share out the steps: two a CU
+constexpr int SHARED_TILES = 1024;     // tiles whose work is shared out evenly; more are enough units by themselves
+constexpr int UNIT_STEPS = 6;          // what a unit costs beside its steps (queries, the first loads, the end), in steps
+
+struct Plan {
+    int ps, per;                       // log2 of the page size; query heads of a key head
+    uint32_t magic;                    // 2^32 / per, rounded up (per > 1)
+    int cols, cblocks;                 // columns of a block, and the blocks of a full tile
+    int groups;                        // few columns: workgroups that the steps are shared out to; 0: a workgroup takes all keys of its unit
+    int runs, run;                     // many columns (cols = 128): key runs of a unit and their steps
+};
+// what `part` holds.  Few columns: the sums of the tiles' costs (int32 [n_tiles + 1]) and a workgroup's share, then for two results of each workgroup [cols][dim] and [cols][2];
+// many columns: the same of each run of each unit
+__host__ __device__ inline int64_t head_floats(int n_tiles) { return ((int64_t)n_tiles + 2 + 3) / 4 * 4; }
+
+// x / per for x per < 2^32
+__device__ __forceinline__ int row_of(const Plan& pl, int x) { return pl.per == 1 ? x : (int)__umulhi((uint32_t)x, pl.magic); }
+
+// e^x of differences of running maxima, in the units that the type keeps them in
+template <typename E>
+__device__ __forceinline__ float pow_of(float x) { return __builtin_amdgcn_exp2f(sizeof(E) == 4 ? x * LOG2E : x); }
+
+// e^(x - M) of an fp32 score: 2^(d log2 e) with log2 e in two parts, so that the error does not grow with |d|
+__device__ __forceinline__ float exp_of_score(float x, float M) {
+    const float d = __builtin_fmaxf(x - M, -200.0f);
+    const float p = d * 1.44269502e+00f, rest = __builtin_fmaf(d, 1.92596303e-08f, __builtin_fmaf(d, 1.44269502e+00f, -p));
+    const float q = __builtin_amdgcn_exp2f(p);
+    return x == NEG ? 0.0f : x == x ? __builtin_fmaf(q, rest * 6.93147182e-01f, q) : x;
+}
+
+// the quotient of a column: its sums under the maximum m, and the sink.  No score above -infinity: 0, but scores that are no numbers stay so
+template <typename E>
+__device__ __forceinline__ float finished(const pcb_attn_pages_args& a, int h, float m, float den, float num) {
+    if (m == NEG) return den * 0.0f;
+    if (a.sink) den += __builtin_amdgcn_exp2f(sizeof(E) == 4 ? (a.sink[h] - m) * LOG2E : a.sink[h] * LOG2E - m);
+    return num * (1.0f / 16384.0f) / den;
+}
+
+// a tile as the kernels take it: no rows where it is of no sequence or reaches out of the rows; and the steps of 64 keys [s0, s1) that some of its rows see
+struct Tile {
+    int seq, pos, rows, row0, kv, s0, s1;
+};
+// the tile with the steps that its rows first .. last see
+__device__ __forceinline__ Tile rows_of(const pcb_attn_pages_args& a, Tile x, int first, int last) {
+    const int end = (int)min((int64_t)x.kv, (int64_t)x.pos + last + 1);
+    int begin = a.window > 0 ? x.pos + first - a.window + 1 : 0;
+    begin = begin < 0 ? 0 : begin;
+    x.s0 = begin >> 6, x.s1 = end > begin ? (end + 63) >> 6 : x.s0;
+    return x;
+}
+__device__ __forceinline__ Tile tile_of(const pcb_attn_pages_args& a, int t, int ps) {
+    const int4 r = reinterpret_cast<const int4*>(a.tiles)[t];
+    Tile x;
+    x.seq = r.x, x.pos = r.y, x.rows = r.z < a.tile_rows ? r.z : a.tile_rows, x.row0 = r.w;
+    x.kv = 0, x.s0 = 0, x.s1 = 0;
+    if (r.x < 0 || r.x >= a.n_seqs || r.y < 0 || r.w < 0 || x.rows <= 0 || (int64_t)r.w + x.rows > a.n_rows) {
+        x.rows = 0;
+        return x;
+    }
+    x.kv = (int)min((int64_t)a.kv_len[r.x], (int64_t)a.max_pages << ps);
+    return rows_of(a, x, 0, x.rows - 1);
+}
+
+}  // namespace pcb
+
+// tiles of many columns (pb_attn_pages_prompt.hip)
+int pcb_attn_pages_prompt(const pcb_attn_pages_args& a, const pcb::Plan& pl, hipStream_t stream);
+#endif

@@ -10,20 +10,10 @@
 // A step walks 64 keys.  Lane group g (16 lanes) owns the sixteen keys 16 g .. 16 g + 15 of the step, in every role: which key a row of the first product's operand is may
 // be chosen freely, so row 4 g + r of its block b is key 16 g + 4 b + r, and the lane's scores are then, in order, the keys of its operand of the second product, sixteen
 // neighbouring codes of a value column, one 16-byte load.  Pages have at least 16 tokens: a lane needs one page number and one pair of scales a step.
-#include "pb_pages.h"
+#include "pb_attn_pages.h"
 
 namespace {
 using namespace pcb;
-
-constexpr float LOG2E = 1.44269504088896f;
-constexpr float NEG = -__builtin_inff();
-
-constexpr int MAX_RUNS = 256;
-
-struct Plan {
-    int ps, per, n_splits, run;        // log2 of the page size; query heads of a key head; key runs and their length in steps of 64 keys
-    int cols, cblocks;                 // columns of a block, and a tile's blocks
-};
 
 __device__ __forceinline__ float max4(float v) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -86,33 +76,6 @@ __device__ __forceinline__ float load_query(const E* p, int dim, int g, bool liv
     return unit;
 }
 
-// e^x of differences of running maxima, in the units that the type keeps them in
-template <typename E>
-__device__ __forceinline__ float pow_of(float x) { return __builtin_amdgcn_exp2f(sizeof(E) == 4 ? x * LOG2E : x); }
-
-// the quotient of a column: its sums under the maximum m, and the sink.  No score above -infinity: 0, but scores that are no numbers stay so
-template <typename E>
-__device__ __forceinline__ float finished(const pcb_attn_pages_args& a, int h, float m, float den, float num) {
-    if (m == NEG) return den * 0.0f;
-    if (a.sink) den += __builtin_amdgcn_exp2f(sizeof(E) == 4 ? (a.sink[h] - m) * LOG2E : a.sink[h] * LOG2E - m);
-    return num * (1.0f / 16384.0f) / den;
-}
-
-// the steps of 64 keys that some of the columns [first, last] of a tile see, and the keys that all of them do
-struct Span {
-    int s0, s1, all_lo, all_hi;
-};
-__device__ __forceinline__ Span span_of(const pcb_attn_pages_args& a, const int4& tile, int kv, int first, int last, int per) {
-    const int p0 = tile.y + first / per, p1 = tile.y + last / per;
-    const int end = min(kv, p1 + 1);
-    int begin = a.window > 0 ? p0 - a.window + 1 : 0;
-    begin = begin < 0 ? 0 : begin;
-    Span s;
-    s.s0 = begin >> 6, s.s1 = end > begin ? (end + 63) >> 6 : s.s0;
-    s.all_lo = a.window > 0 ? p1 - a.window + 1 : 0, s.all_hi = min(kv, p0 + 1);
-    return s;
-}
-
 // Sixteen scores of a lane (in units of 1 / f; -infinity: not seen) as weights of the second product: w = e^(s - M) vs 2^14 with M the running maximum of s + ln vs over the
 // column's keys; l += the lane's part of sum e^(s - M); alpha: what earlier results are multiplied with.
 template <typename E, int PARTS>
@@ -140,11 +103,7 @@ __device__ __forceinline__ void weights(f4 (&acc)[4], float f, float vs, float& 
         const float up = vs * 16384.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            // 2^(d log2 e) with log2 e in two parts: the error does not grow with |d|
-            const float x = acc[i >> 2][i & 3] * f, d = __builtin_fmaxf(x - M_use, -200.0f);
-            const float p = d * 1.44269502e+00f, rest = __builtin_fmaf(d, 1.92596303e-08f, __builtin_fmaf(d, 1.44269502e+00f, -p));
-            const float q = __builtin_amdgcn_exp2f(p);
-            const float e = x == NEG ? 0.0f : x == x ? __builtin_fmaf(q, rest * 6.93147182e-01f, q) : x;
+            const float e = exp_of_score(acc[i >> 2][i & 3] * f, M_use);
             sum += e;
             const float w = e * up;
             const _Float16 top16 = (_Float16)w;
@@ -155,305 +114,391 @@ __device__ __forceinline__ void weights(f4 (&acc)[4], float f, float vs, float& 
     l = l * alpha + sum;
 }
 
-// A workgroup: 16 NC columns of a tile and key head, a run of its keys, which the waves take step by step in turns.  A wave's keys and values go from memory straight
-// into operand registers, and the next step's are asked for as soon as this one's have been multiplied: nothing crosses waves but the end.
-template <typename E, int CODE, int DB, int NC, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn_pages_rows_kernel(pcb_attn_pages_args a, Plan pl) {
+// A unit is 16 NC columns of a tile and one key head.  The steps of all units, one after the other, are shared out evenly: a workgroup's share may begin inside a unit and
+// end inside another one; what is not a whole unit goes to `part`.  So sequences of any lengths fill the chip alike, and no workgroup starts in vain.  A unit without steps
+// counts as one: its rows get their zeros.
+//
+// Within a unit the waves take steps in turns.  Keys and values go from memory straight into operand registers: a step's values are under way during its softmax, the next
+// step's keys as soon as this one's values have been multiplied, and the two take turns in the same registers; nothing crosses waves but the end.  (Both with registers of
+// their own, a step ahead: no faster with two workgroups a CU, and the same with three or four, which their registers then only allow with spills, 1.1 to 1.6 x the time.)
+template <typename E, int CODE, int DB, int NC>
+__global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_args a, Plan pl) {
     constexpr bool F32 = sizeof(E) == 4;
-    constexpr int PARTS = F32 ? 2 : 1, NB = 4 * DB;                 // value column blocks of 16
-    __shared__ float Os[NW][NB * 16][17];
-    __shared__ float Ms[NW][16 * NC], Ls[NW][16 * NC];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
-    const int t = blockIdx.x, z = blockIdx.z, hk = blockIdx.y / pl.cblocks, cb = blockIdx.y % pl.cblocks;
-    const int4 tile = reinterpret_cast<const int4*>(a.tiles)[t];
-    const int seq = tile.x;
-    if (seq < 0 || seq >= a.n_seqs) return;
-    int rows = tile.z < a.tile_rows ? tile.z : a.tile_rows;
-    if (tile.w < 0 || tile.y < 0 || (int64_t)tile.w + rows > a.n_rows) rows = 0;
-    const int per = pl.per, col0 = cb * 16 * NC, dim = a.dim, ps = pl.ps, P = 1 << ps;
-    if (col0 >= rows * per) return;
-    int kv = a.kv_len[seq];
-    kv = (int)min((int64_t)kv, (int64_t)a.max_pages << ps);
-    const Span sp = span_of(a, tile, kv, col0, min(col0 + 16 * NC, rows * per) - 1, per);
-    int s0 = sp.s0, s1 = sp.s1;
-    const bool split = pl.n_splits > 1 && s1 - s0 > pl.run;           // (what one run holds is finished here)
-    if (split) {
-        s0 += z * pl.run;
-        if (z < pl.n_splits - 1) s1 = min(s1, s0 + pl.run);
-        if (s0 >= s1) return;
-    } else if (z > 0) {
-        return;
-    }
-    int lo[NC], hi[NC];                                               // a column's keys [lo, hi)
-    float qs[NC];
-    h8 qf[NC][PARTS][2 * DB];
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        const int col = col0 + 16 * n + c, qr = col / per;
-        const bool live = col < rows * per;
-        const int pos = live ? tile.y + qr : -1, h = hk * per + (live ? col % per : 0);
-        lo[n] = a.window > 0 ? pos - a.window + 1 : 0, hi[n] = min(kv, pos + 1);
-        const float unit =
-            load_query<E, DB, PARTS>((const E*)a.q + ((int64_t)tile.w + (live ? qr : 0)) * a.ldq + (int64_t)h * a.q_head_stride, dim, g, live, qf[n]);
-        qs[n] = F32 ? unit * a.scale : unit * (a.scale * LOG2E);      // bf16: scores in units of ln 2
-    }
-    const int32_t* table = a.table + (int64_t)seq * a.ld_table;
+    constexpr int NW = 4, NT = 256, PARTS = F32 ? 2 : 1, NB = 4 * DB, COLS = 16 * NC;   // NB: value column blocks of 16
+    __shared__ __attribute__((aligned(16))) float Os[NW][16][64 * DB + 4];
+    __shared__ float Ms[NW][COLS], Ls[NW][COLS];
+    __shared__ int starts[SHARED_TILES + 1], wsum[NW];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int per = pl.per, dim = a.dim, ps = pl.ps, P = 1 << ps;
     const int64_t plane = (int64_t)P * dim;
-    const bool whole = dim == 64 * DB;
-    float M[NC], l[NC];
-    f4 o[NC][NB];
+    // Heads of less than 64 DB elements: what lies behind reads a head's last sixteen again (numbers, times the queries' zeros) or a column block that nobody stores
+    const int last_b = dim / 16 - 1;
+    int at = 0, end = 1, share = 1;
+    if (pl.groups) {
+        const int tid = threadIdx.x, lane = tid & 63;
+        int all = 0;
+        for (int t0 = 0; t0 < a.n_tiles; t0 += NT) {
+            int n = 0;
+            if (t0 + tid < a.n_tiles) {
+                const Tile x = tile_of(a, t0 + tid, ps);
+                n = (max(x.s1 - x.s0, 1) + UNIT_STEPS) * a.Hkv * ((x.rows * per + COLS - 1) / COLS);
+            }
+            int v = n;
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        M[n] = NEG, l[n] = 0.0f;
+            for (int o = 1; o < 64; o <<= 1) {
+                const int u = __shfl_up(v, o, 64);
+                if (lane >= o) v += u;
+            }
+            if (lane == 63) wsum[wave] = v;
+            __syncthreads();
+            int sum = 0;
 #pragma unroll
-        for (int i = 0; i < NB; ++i) o[n][i] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int w = 0; w < NW; ++w) {
+                if (w < wave) v += wsum[w];
+                sum += wsum[w];
+            }
+            if (t0 + tid < a.n_tiles) starts[t0 + tid] = all + v - n;
+            all += sum;
+            __syncthreads();
+        }
+        all = __builtin_amdgcn_readfirstlane(all);
+        share = (all + pl.groups - 1) / pl.groups;
+        share = share < NW + UNIT_STEPS ? NW + UNIT_STEPS : share;
+        if (tid == 0) starts[a.n_tiles] = all;
+        __syncthreads();
+        if (blockIdx.x == 0) {                                        // for the launch that merges
+            int* head = reinterpret_cast<int*>(a.part);
+            for (int t = tid; t <= a.n_tiles; t += NT) head[t] = starts[t];
+            if (tid == 0) head[a.n_tiles + 1] = share;
+        }
+        at = blockIdx.x * share, end = min(at + share, all);
     }
-    // pages and scales of sixteen of the wave's steps at once: lane 4 i + k those of its step i's keys 16 k ..
-    int pages = -1;
-    float kss = 1.0f, vss = 1.0f;
-    auto look = [&](int s) {
-        const int key = (s + (lane >> 2) * NW) * 64 + 16 * (lane & 3);
-        pages = s + (lane >> 2) * NW < s1 && key < kv ? table[key >> ps] : -1;
-        pages = pages >= 0 && pages < a.n_pages ? pages : -1;
-        const int64_t ph = (int64_t)(pages < 0 ? 0 : pages) * a.Hkv + hk;
-        kss = pages < 0 ? 1.0f : a.kscale[ph], vss = pages < 0 ? 1.0f : a.vscale[ph];
-    };
-    u32x4 kr[4][DB], vr[NB];
-    auto fetch_k = [&](int s, int i) {
-        const int page = __shfl(pages, 4 * i + (c >> 2), 64);         // of the sixteen keys that row c of the first product's operand is one of
-        const int row = ((s * 64 + 16 * (c >> 2)) & (P - 1)) + (c & 3);
-        const uint8_t* p = (const uint8_t*)a.kcodes + ((int64_t)(page < 0 ? 0 : page) * a.Hkv + hk) * plane + row * dim + 16 * g;
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int ch = 0; ch < DB; ++ch) {
-                if (whole || 64 * ch + 16 * g < dim)
-                    kr[b][ch] = *reinterpret_cast<const u32x4*>(p + 4 * b * dim + 64 * ch);
+    const int at0 = at;
+    float* const part = a.part + head_floats(a.n_tiles);
+    while (at < end) {
+        int t, j, from, steps, n_steps, mine = 1;                     // unit j of tile t, its steps from .. from + n_steps - 1
+        Tile tl;
+        if (pl.groups) {
+            int lo = 0, hi = a.n_tiles;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (starts[mid] <= at)
+                    lo = mid;
                 else
-                    kr[b][ch] = u32x4{0u, 0u, 0u, 0u};
+                    hi = mid;
             }
-    };
-    auto fetch_v = [&](int s, int i) {
-        const int page = __shfl(pages, 4 * i + g, 64);
-        const uint8_t* p = (const uint8_t*)a.vcodes + ((int64_t)(page < 0 ? 0 : page) * a.Hkv + hk) * plane + ((s * 64 + 16 * g) & (P - 1)) + c * P;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-            if (16 * b < dim) vr[b] = *reinterpret_cast<const u32x4*>(p + 16 * b * P);
-    };
-    int s = s0 + wave, i = 0;
-    if (s < s1) {
-        look(s);
-        fetch_k(s, 0);
-        fetch_v(s, 0);
-    }
-    for (; s < s1; s += NW) {
-        f4 acc[NC][4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-#pragma unroll
-            for (int n = 0; n < NC; ++n) acc[n][b] = f4{0.f, 0.f, 0.f, 0.f};
+            t = __builtin_amdgcn_readfirstlane(lo);
+            tl = tile_of(a, t, ps);
+            steps = max(tl.s1 - tl.s0, 1);
+            const int off = at - __builtin_amdgcn_readfirstlane(starts[t]), cost = steps + UNIT_STEPS;
+            j = off / cost;
+            const int p = off - j * cost;
+            mine = min(cost - p, end - at);
+            from = max(p - UNIT_STEPS, 0), n_steps = max(p + mine - UNIT_STEPS, 0) - from;
+        } else {
+            t = blockIdx.x, j = blockIdx.y;
+            tl = tile_of(a, t, ps);
+            from = 0, steps = n_steps = max(tl.s1 - tl.s0, 1);
+            if (j / a.Hkv * COLS >= tl.rows * per) return;
+        }
+        const bool unit = n_steps == steps;
+        const int slot = unit ? 0 : 2 * (int)blockIdx.x + (at == at0 ? 0 : 1);
+        at += mine;
+        if (n_steps == 0) continue;                                   // (the share ends before the unit's first step)
+        int tid = threadIdx.x;
+        asm("" : "+v"(tid));                                          // (what hangs on it is computed anew for every unit: kept over the loop it takes the inner one's registers)
+        const int lane = tid & 63, g = lane >> 4, c = lane & 15;
+        const int cblock = j / a.Hkv, hk = j - cblock * a.Hkv, col0 = cblock * COLS, rows = tl.rows, kv = tl.kv;
+        const int s0 = tl.s0 + from, s1 = min(s0 + n_steps, tl.s1);
+        const int last_col = min(col0 + COLS, rows * per) - 1;
+        // keys that all of the unit's columns see
+        const int all_lo = a.window > 0 ? tl.pos + row_of(pl, last_col) - a.window + 1 : 0, all_hi = min(kv, tl.pos + row_of(pl, col0) + 1);
+        int lo[NC], hi[NC];                                           // a column's keys [lo, hi)
+        float qs[NC];
+        h8 qf[NC][PARTS][2 * DB];
+        const int32_t* table = a.table + (int64_t)tl.seq * a.ld_table;
+        // pages and scales of sixteen of the wave's steps at once: lane 4 i + k those of its step i's keys 16 k ..
+        int pages = -1;
+        float kss = 1.0f, vss = 1.0f;
+        auto look = [&](int s) {
+            const int key = (s + (lane >> 2) * NW) * 64 + 16 * (lane & 3);
+            pages = s + (lane >> 2) * NW < s1 && key < kv ? table[key >> ps] : -1;
+            pages = pages >= 0 && pages < a.n_pages ? pages : -1;
+            const int64_t ph = (int64_t)(pages < 0 ? 0 : pages) * a.Hkv + hk;
+            kss = pages < 0 ? 1.0f : a.kscale[ph], vss = pages < 0 ? 1.0f : a.vscale[ph];
+        };
+        u32x4 kr[4][DB], vr[NB];
+        auto fetch_k = [&](int s, int i) {
+            const int page = __shfl(pages, 4 * i + (c >> 2), 64);     // of the sixteen keys that row c of the first product's operand is one of
+            const int row = ((s * 64 + 16 * (c >> 2)) & (P - 1)) + (c & 3);
+            const uint8_t* p = (const uint8_t*)a.kcodes + ((int64_t)(page < 0 ? 0 : page) * a.Hkv + hk) * plane + row * dim;
 #pragma unroll
             for (int ch = 0; ch < DB; ++ch) {
-                const h8 k0 = half8<CODE>(u32x2{kr[b][ch][0], kr[b][ch][1]}), k1 = half8<CODE>(u32x2{kr[b][ch][2], kr[b][ch][3]});
+                const uint8_t* q = p + 16 * min(4 * ch + g, last_b);
+                asm("" : "+v"(q));                                    // (one address and steps that all lanes share, not sixteen sums kept over the loop)
 #pragma unroll
-                for (int n = 0; n < NC; ++n)
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        acc[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qf[n][p][2 * ch], acc[n][b], 0, 0, 0);
-                        acc[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qf[n][p][2 * ch + 1], acc[n][b], 0, 0, 0);
-                    }
+                for (int b = 0; b < 4; ++b) kr[b][ch] = *reinterpret_cast<const u32x4*>(q + 4 * b * dim);
             }
+        };
+        auto fetch_v = [&](int s, int i) {
+            const int page = __shfl(pages, 4 * i + g, 64);
+            const uint8_t* p = (const uint8_t*)a.vcodes + ((int64_t)(page < 0 ? 0 : page) * a.Hkv + hk) * plane + ((s * 64 + 16 * g) & (P - 1)) + c * P;
+            asm("" : "+v"(p));
+#pragma unroll
+            for (int b = 0; b < NB; ++b) vr[b] = *reinterpret_cast<const u32x4*>(p + 16 * min(b, last_b) * P);
+        };
+        int s = s0 + wave, i = 0;
+        if (s < s1) {
+            look(s);
+            fetch_k(s, 0);
         }
-        const int key0 = s * 64 + 16 * g;
-        const int page = __shfl(pages, 4 * i + g, 64);
-        const float ks = __shfl(kss, 4 * i + g, 64), vs = __shfl(vss, 4 * i + g, 64);
-        const bool more = s + NW < s1;
-        const int i_next = (i + 1) & 15;
-        if (more) {
-            if (i_next == 0) look(s + NW);
-            fetch_k(s + NW, i_next);
-        }
-        // a step that all columns see whole needs no comparisons
-        const bool seen = s * 64 + 64 <= sp.all_hi && s * 64 >= sp.all_lo && __all(page >= 0);
-        h8 wf[NC][PARTS][2];
-        float alpha[NC];
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            if (!seen) {
+            const int col = col0 + 16 * n + c;
+            const bool live = col < rows * per;
+            const int qr = live ? row_of(pl, col) : 0, h = hk * per + (live ? col - qr * per : 0), pos = live ? tl.pos + qr : -1;
+            lo[n] = a.window > 0 ? pos - a.window + 1 : 0, hi[n] = min(kv, pos + 1);
+            const float unit2 = load_query<E, DB, PARTS>((const E*)a.q + ((int64_t)tl.row0 + qr) * a.ldq + (int64_t)h * a.q_head_stride, dim, g, live, qf[n]);
+            qs[n] = F32 ? unit2 * a.scale : unit2 * (a.scale * LOG2E);  // bf16: scores in units of ln 2
+        }
+        float M[NC], l[NC];
+        f4 o[NC][NB];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = key0 + e;
-                    if (!(page >= 0 && key >= lo[n] && key < hi[n])) acc[n][e >> 2][e & 3] = NEG;
+        for (int n = 0; n < NC; ++n) {
+            M[n] = NEG, l[n] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) o[n][b] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+        for (; s < s1; s += NW) {
+            f4 acc[NC][4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n) acc[n][b] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ch = 0; ch < DB; ++ch) {
+                    const h8 k0 = half8<CODE>(u32x2{kr[b][ch][0], kr[b][ch][1]}), k1 = half8<CODE>(u32x2{kr[b][ch][2], kr[b][ch][3]});
+#pragma unroll
+                    for (int n = 0; n < NC; ++n)
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            acc[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qf[n][p][2 * ch], acc[n][b], 0, 0, 0);
+                            acc[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qf[n][p][2 * ch + 1], acc[n][b], 0, 0, 0);
+                        }
                 }
             }
-            weights<E, PARTS>(acc[n], qs[n] * ks, vs, M[n], l[n], alpha[n], wf[n]);
-        }
-        // values: codes behind the last written key are whatever the memory held, and no number times 0 is 0 for all of them
-        if (!seen) {
-            const int have = page < 0 ? 0 : kv - key0;
+            const int key0 = s * 64 + 16 * g;
+            const int page = __shfl(pages, 4 * i + g, 64);
+            const float ks = __shfl(kss, 4 * i + g, 64), vs = __shfl(vss, 4 * i + g, 64);
+            const bool more = s + NW < s1;
+            const int i_next = (i + 1) & 15;
+            __builtin_amdgcn_sched_barrier(0);                        // (the phases' registers do not overlap; loads drawn ahead into the one before would make them)
+            fetch_v(s, i);
+            // a step that all columns see whole needs no comparisons
+            const bool seen = s * 64 + 64 <= all_hi && s * 64 >= all_lo && __all(page >= 0);
+            h8 wf[NC][PARTS][2];
+            float alpha[NC];
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int n = 0; n < NC; ++n) {
+                if (!seen) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = key0 + e;
+                        if (!(page >= 0 && key >= lo[n] && key < hi[n])) acc[n][e >> 2][e & 3] = NEG;
+                    }
+                }
+                weights<E, PARTS>(acc[n], qs[n] * ks, vs, M[n], l[n], alpha[n], wf[n]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // values: codes behind the last written key are whatever the memory held, and no number times 0 is 0 for all of them
+            if (!seen) {
+                const int have = page < 0 ? 0 : kv - key0;
+                uint32_t keep[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int k = have - 4 * e;
-                    vr[b][e] &= k >= 4 ? 0xffffffffu : k <= 0 ? 0u : 0xffffffffu >> (32 - 8 * k);
+                    keep[e] = k >= 4 ? 0xffffffffu : k <= 0 ? 0u : 0xffffffffu >> (32 - 8 * k);
                 }
-        }
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if (16 * b >= dim) continue;
-            const h8 v0 = half8<CODE>(u32x2{vr[b][0], vr[b][1]}), v1 = half8<CODE>(u32x2{vr[b][2], vr[b][3]});
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int n = 0; n < NC; ++n) {
+                    for (int e = 0; e < 4; ++e) vr[b][e] &= keep[e];
+            }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[n][b][r] *= alpha[n];
+            for (int b = 0; b < NB; ++b) {
+                const h8 v0 = half8<CODE>(u32x2{vr[b][0], vr[b][1]}), v1 = half8<CODE>(u32x2{vr[b][2], vr[b][3]});
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
-                    o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, wf[n][p][0], o[n][b], 0, 0, 0);
-                    o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, wf[n][p][1], o[n][b], 0, 0, 0);
+                for (int n = 0; n < NC; ++n) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[n][b][r] *= alpha[n];
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, wf[n][p][0], o[n][b], 0, 0, 0);
+                        o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, wf[n][p][1], o[n][b], 0, 0, 0);
+                    }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) {
+                if (i_next == 0) look(s + NW);
+                fetch_k(s + NW, i_next);
+            }
+            i = i_next;
         }
-        if (more) fetch_v(s + NW, i_next);
-        i = i_next;
-    }
-    // the waves' results under one maximum, sixteen columns after sixteen
+        // the waves' results under one maximum, sixteen columns after sixteen: sixteen threads a column, four neighbouring elements each
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        l[n] = sum4(l[n]);
-        if (g == 0) Ms[wave][16 * n + c] = M[n], Ls[wave][16 * n + c] = l[n];
-    }
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        __syncthreads();
-        float top = NEG;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) top = fmaxf(top, Ms[w][16 * n + c]);
-        const float back = pow_of<E>(M[n] - (top == NEG ? 0.0f : top));
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if (16 * b >= dim) continue;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) Os[wave][16 * b + 4 * g + r][c] = o[n][b][r] * back;
+        for (int n = 0; n < NC; ++n) {
+            l[n] = sum4(l[n]);
+            if (g == 0) Ms[wave][16 * n + c] = M[n], Ls[wave][16 * n + c] = l[n];
         }
-        __syncthreads();
-        const int first = col0 + 16 * n, n_live = min(16, rows * per - first);
-        for (int e = tid; e < n_live * dim; e += 64 * NW) {
-            const int cc = e / dim, d = e - cc * dim;
-            float m = NEG, den = 0.0f, num = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            __syncthreads();
+            float top = NEG;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) top = fmaxf(top, Ms[w][16 * n + c]);
+            const float back = pow_of<E>(M[n] - (top == NEG ? 0.0f : top));
+#pragma unroll
+            for (int b = 0; b < NB; ++b) *reinterpret_cast<f4*>(&Os[wave][c][16 * b + 4 * g]) = o[n][b] * back;
+            __syncthreads();
+            const int cc = tid >> 4, col = col0 + 16 * n + cc;
+            if (col >= rows * per) continue;
+            float m = NEG, den = 0.0f;
 #pragma unroll
             for (int w = 0; w < NW; ++w) m = fmaxf(m, Ms[w][16 * n + cc]);
-            const float mu = m == NEG ? 0.0f : m;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                den += Ls[w][16 * n + cc] * pow_of<E>(Ms[w][16 * n + cc] - mu);
-                num += Os[w][d][cc];
-            }
-            const int cl = first + cc, hh = hk * per + cl % per;
-            const int64_t row = (int64_t)tile.w + cl / per;
-            if (split) {
-                const int64_t at = (row * a.H + hh) * pl.n_splits + z;
-                a.part[at * dim + d] = num;
-                if (d == 0) *reinterpret_cast<float2*>(a.part + (int64_t)a.n_rows * a.H * pl.n_splits * dim + 2 * at) = float2{m, den};
-            } else {
-                ((E*)a.out)[row * a.ldo + (int64_t)hh * a.out_head_stride + d] = from_f32<E>(finished<E>(a, hh, m, den, num));
+            for (int w = 0; w < NW; ++w) den += Ls[w][16 * n + cc] * pow_of<E>(Ms[w][16 * n + cc] - (m == NEG ? 0.0f : m));
+            const int qr = row_of(pl, col), h = hk * per + col - qr * per;
+            float* pp = part + (int64_t)slot * COLS * (dim + 2);
+            E* op = (E*)a.out + ((int64_t)tl.row0 + qr) * a.ldo + (int64_t)h * a.out_head_stride;
+            const float f = unit ? finished<E>(a, h, m, den, 16384.0f) * (1.0f / 16384.0f) : 1.0f;
+            if (!unit && (tid & 15) == 0) *reinterpret_cast<float2*>(pp + COLS * dim + 2 * (16 * n + cc)) = float2{m, den};
+            for (int d = 4 * (tid & 15); d < dim; d += 64) {
+                f4 v = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < NW; ++w) v += *reinterpret_cast<const f4*>(&Os[w][cc][d]);
+                if (unit)
+                    store4(op + d, v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+                else
+                    *reinterpret_cast<f4*>(pp + (16 * n + cc) * dim + d) = v;
             }
         }
+        __syncthreads();
     }
 }
 
-// One workgroup a (tile, head): the key runs' results under one maximum.  The runs' factors once (a lane a run), then groups of dim / 4 threads add up every so many runs.
+// One workgroup a (tile, head, row): the results of the workgroups that shared the row's unit under one maximum.  Their factors once (a lane each), then groups of dim / 4 threads
+// add up every so many of them.
 template <typename E>
 __global__ __launch_bounds__(256) void attn_pages_merge_kernel(pcb_attn_pages_args a, Plan pl) {
-    __shared__ float fac[MAX_RUNS];
+    __shared__ float fac[MAX_GROUPS];
     __shared__ f4 sums[256];
-    __shared__ float den_s;
-    const int4 tile = reinterpret_cast<const int4*>(a.tiles)[blockIdx.x];
-    const int seq = tile.x, h = blockIdx.y, dim = a.dim, tid = threadIdx.x, lane = tid & 63;
-    if (seq < 0 || seq >= a.n_seqs) return;
-    int rows = tile.z < a.tile_rows ? tile.z : a.tile_rows;
-    if (tile.w < 0 || tile.y < 0 || (int64_t)tile.w + rows > a.n_rows) rows = 0;
-    int kv = a.kv_len[seq];
-    kv = (int)min((int64_t)kv, (int64_t)a.max_pages << pl.ps);
+    __shared__ float inv_s;
+    const int h = blockIdx.y, dim = a.dim, tid = threadIdx.x, lane = tid & 63, t = blockIdx.x;
+    const Tile tl = tile_of(a, t, pl.ps);
     const int per = pl.per, quads = dim / 4, groups = 256 / quads, grp = tid / quads, quad = tid % quads;
-    const float* ml = a.part + (int64_t)a.n_rows * a.H * pl.n_splits * dim;
-    for (int r = blockIdx.z; r < rows; r += gridDim.z) {
-        const int first = (r * per + h % per) / pl.cols * pl.cols;
-        const Span sp = span_of(a, tile, kv, first, min(first + pl.cols, rows * per) - 1, per);   // what the row's column block walked
-        if (sp.s1 - sp.s0 <= pl.run) continue;
-        const int n = min(pl.n_splits, (sp.s1 - sp.s0 + pl.run - 1) / pl.run);
-        const int64_t row = (int64_t)tile.w + r, at = (row * a.H + h) * pl.n_splits;
+    const bool many = pl.cols == MANY_COLS;
+    const int* head = reinterpret_cast<const int*>(a.part);
+    const int start = many ? 0 : head[t], share = many ? 1 : head[a.n_tiles + 1];
+    const float* part = many ? a.part : a.part + head_floats(a.n_tiles);
+    const int64_t result = (int64_t)pl.cols * (dim + 2);
+    for (int r = blockIdx.z; r < tl.rows; r += gridDim.z) {
+        const int col = r * per + h % per, cc = col % pl.cols, cblock = col / pl.cols, hk = h / per;
+        int64_t first;                                                // the place of the unit's first result, and that of its second
+        int64_t second;
+        int n;
+        if (many) {
+            const Tile bl = rows_of(a, tl, row_of(pl, cblock * MANY_COLS), row_of(pl, min(cblock * MANY_COLS + MANY_COLS, tl.rows * per) - 1));
+            n = min((bl.s1 - bl.s0 + pl.run - 1) / pl.run, pl.runs);
+            first = (((int64_t)t * a.Hkv + hk) * pl.cblocks + cblock) * pl.runs, second = first + 1;
+        } else {
+            const int steps = max(tl.s1 - tl.s0, 1), u0 = start + (steps + UNIT_STEPS) * (cblock * a.Hkv + hk), s0 = u0 + UNIT_STEPS;   // the unit's and its first step's place among all
+            const int g0 = s0 / share;
+            n = (s0 + steps - 1) / share - g0 + 1;
+            first = 2 * (int64_t)g0 + (u0 > g0 * share ? 1 : 0), second = 2 * ((int64_t)g0 + 1);
+        }
+        if (n <= 1) continue;                                         // (one workgroup had it all)
+        const int64_t apart = many ? 1 : 2;
+        auto place = [&](int i) { return part + (i == 0 ? first : second + apart * (i - 1)) * result; };
         __syncthreads();
         if (tid < 64) {
-            float m = NEG;
-            for (int i = lane; i < n; i += 64) m = fmaxf(m, ml[2 * (at + i)]);
+            float m = NEG, den = 0.0f;
+            for (int i = lane; i < n; i += 64) m = fmaxf(m, place(i)[pl.cols * dim + 2 * cc]);
             m = wave_max(m);
             const float mu = m == NEG ? 0.0f : m;
-            float den = 0.0f;
             for (int i = lane; i < n; i += 64) {
-                const float2 x = *reinterpret_cast<const float2*>(ml + 2 * (at + i));
+                const float2 x = *reinterpret_cast<const float2*>(place(i) + pl.cols * dim + 2 * cc);
                 const float f = pow_of<E>(x.x - mu);
                 fac[i] = f;
                 den += x.y * f;
             }
             den = wave_sum(den);
-            if (lane == 0) den_s = finished<E>(a, h, m, den, 16384.0f);
+            if (lane == 0) inv_s = finished<E>(a, h, m, den, 16384.0f);
         }
         __syncthreads();
         f4 v = f4{0.f, 0.f, 0.f, 0.f};
         if (grp < groups)
 #pragma unroll 4
-            for (int i = grp; i < n; i += groups) v += *reinterpret_cast<const f4*>(a.part + (at + i) * dim + 4 * quad) * fac[i];
+            for (int i = grp; i < n; i += groups) v += *reinterpret_cast<const f4*>(place(i) + cc * dim + 4 * quad) * fac[i];
         sums[tid] = v;
         __syncthreads();
         if (tid < quads) {
             for (int k = 1; k < groups; ++k) v += sums[k * quads + quad];
-            v *= den_s * (1.0f / 16384.0f);
-            store4((E*)a.out + row * a.ldo + (int64_t)h * a.out_head_stride + 4 * quad, v[0], v[1], v[2], v[3]);
+            v *= inv_s * (1.0f / 16384.0f);
+            store4((E*)a.out + ((int64_t)tl.row0 + r) * a.ldo + (int64_t)h * a.out_head_stride + 4 * quad, v[0], v[1], v[2], v[3]);
         }
     }
 }
 
-// How a call is cut.  Columns: what a tile has, in blocks of 16 or 32.  Key runs: ...
+// How a call is cut.  Up to 32 columns a tile: in blocks of 16 or 32, the steps of everything shared out; more: blocks of 128, in key runs where these are too few to fill
+// the chip.
 Plan plan_of(int64_t H, int Hkv, int dim, int n_tiles, int tile_rows, int64_t longest) {
-    Plan p;
-    p.ps = 0;
+    Plan p{};
     p.per = (int)(H / Hkv);
-    const int64_t cols = (int64_t)tile_rows * p.per;
-    p.cols = cols <= 16 || dim > 128 ? 16 : 32;
+    p.magic = p.per > 1 ? (uint32_t)(((1ull << 32) + p.per - 1) / p.per) : 0;
+    const int64_t cols = (int64_t)tile_rows * p.per, steps = (longest + 63) / 64 > 0 ? (longest + 63) / 64 : 1;
+    p.cols = tile_rows > 1 && cols > 32 ? MANY_COLS : cols <= 16 || dim > 128 ? 16 : 32;
     p.cblocks = (int)(cols > 1 << 30 ? 1 << 26 : (cols + p.cols - 1) / p.cols);
-    const int64_t units = (int64_t)n_tiles * Hkv * p.cblocks, steps = (longest + 63) / 64;
-    int64_t run = (units * steps + 1023) / 1024;
-    run = run < 4 ? 4 : run > 16 ? 16 : run;
-    if (run < units * steps / 4096) run = units * steps / 4096;
-    if (run < (steps + MAX_RUNS - 1) / MAX_RUNS) run = (steps + MAX_RUNS - 1) / MAX_RUNS;
-    if (steps <= 8) run = 8;
-    p.run = (int)run;
-    p.n_splits = (int)((steps + run - 1) / run);
-    if (p.n_splits < 1) p.n_splits = 1;
+    const int64_t units = (int64_t)n_tiles * Hkv * p.cblocks;
+    p.runs = 1, p.run = 1 << 30;
+    if (p.cols == MANY_COLS) {
+        int64_t n = units >= 384 ? 1 : 512 / units;
+        if (n > (steps + 7) / 8) n = (steps + 7) / 8;
+        if (n > 1) p.run = (int)((steps + n - 1) / n), p.runs = (int)((steps + p.run - 1) / p.run);
+    } else if (n_tiles <= SHARED_TILES && steps > 8) {
+        const int64_t fours = (units * steps + 3) / 4;
+        p.groups = (int)(fours < MAX_GROUPS ? fours : MAX_GROUPS);
+    }
     return p;
+}
+int64_t part_floats(const Plan& p, int Hkv, int dim, int n_tiles) {
+    if (p.cols == MANY_COLS) return p.runs > 1 ? (int64_t)n_tiles * Hkv * p.cblocks * p.runs * MANY_COLS * (dim + 2) : 0;
+    return p.groups ? head_floats(n_tiles) + 2 * (int64_t)p.groups * p.cols * (dim + 2) : 0;
 }
 
 template <typename E, int CODE, int DB>
 void launch_rows(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
-    const dim3 grid(a.n_tiles, a.Hkv * pl.cblocks, pl.n_splits), block(256);
+    const dim3 grid(pl.groups ? pl.groups : a.n_tiles, pl.groups ? 1 : a.Hkv * pl.cblocks), block(256);
     if constexpr (DB <= 2)
         if (pl.cols == 32) {
-            hipLaunchKernelGGL((attn_pages_rows_kernel<E, CODE, DB, 2, 4>), grid, block, 0, stream, a, pl);
+            hipLaunchKernelGGL((attn_pages_rows_kernel<E, CODE, DB, 2>), grid, block, 0, stream, a, pl);
             return;
         }
-    hipLaunchKernelGGL((attn_pages_rows_kernel<E, CODE, DB, 1, 4>), grid, block, 0, stream, a, pl);
+    hipLaunchKernelGGL((attn_pages_rows_kernel<E, CODE, DB, 1>), grid, block, 0, stream, a, pl);
 }
 
 template <typename E, int CODE>
 int dispatch(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
-    if (a.dim <= 64)
+    if (pl.cols == MANY_COLS) {
+        const int rc = pcb_attn_pages_prompt(a, pl, stream);
+        if (rc != PCB_OK) return rc;
+    } else if (a.dim <= 64)
         launch_rows<E, CODE, 1>(a, pl, stream);
     else if (a.dim <= 128)
         launch_rows<E, CODE, 2>(a, pl, stream);
     else
         launch_rows<E, CODE, 4>(a, pl, stream);
-    if (pl.n_splits > 1) hipLaunchKernelGGL(attn_pages_merge_kernel<E>, dim3(a.n_tiles, a.H, a.tile_rows < 32 ? a.tile_rows : 32), dim3(256), 0, stream, a, pl);
+    if (pl.groups || pl.runs > 1) hipLaunchKernelGGL(attn_pages_merge_kernel<E>, dim3(a.n_tiles, a.H, a.tile_rows < 32 ? a.tile_rows : 32), dim3(256), 0, stream, a, pl);
     return pcb_check_launch("attn_pages_rows_kernel");
 }
 
@@ -463,7 +508,7 @@ PCB_EXPORT int64_t pcb_attn_pages_part(int32_t n_rows, int32_t H, int32_t Hkv, i
     PCB_REQUIRE(n_rows >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && dim > 0 && n_tiles >= 0 && tile_rows > 0 && longest >= 0, PCB_ERR_ARG, "pcb_attn_pages_part: bad sizes");
     if (n_rows == 0 || n_tiles == 0) return 0;
     const Plan p = plan_of(H, Hkv, dim, n_tiles, tile_rows, longest);
-    return p.n_splits > 1 ? (int64_t)n_rows * H * p.n_splits * (dim + 2) : 0;
+    return part_floats(p, Hkv, dim, n_tiles);
 }
 
 PCB_EXPORT int pcb_attn_pages(const pcb_attn_pages_args* a, void* stream) {
@@ -483,10 +528,12 @@ PCB_EXPORT int pcb_attn_pages(const pcb_attn_pages_args* a, void* stream) {
     const int64_t longest = a->longest > 0 ? a->longest : (int64_t)a->max_pages * a->page_size;
     Plan p = plan_of(a->H, a->Hkv, a->dim, a->n_tiles, a->tile_rows, longest);
     p.ps = pcb_log2(a->page_size);
-    PCB_REQUIRE((int64_t)a->Hkv * p.cblocks <= 65535 && a->H <= 65535 && a->n_tiles < 1 << 23, PCB_ERR_ARG,
-                "pcb_attn_pages: too many tiles, heads or tile rows (heads times tile rows up to 2^20)");
-    PCB_REQUIRE(p.n_splits == 1 || (a->part && (uintptr_t)a->part % 16 == 0 && a->part_floats >= (int64_t)a->n_rows * a->H * p.n_splits * (a->dim + 2)), PCB_ERR_ARG,
-                "pcb_attn_pages: key runs need pcb_attn_pages_part floats");
+    // (costs are counted in 31 bits; whoever has more of them has enough units)
+    if (p.groups && (int64_t)a->n_tiles * a->Hkv * p.cblocks > 0x7fffffff / ((int64_t)a->max_pages * a->page_size / 64 + 2 + UNIT_STEPS) - MAX_GROUPS) p.groups = 0;
+    PCB_REQUIRE((int64_t)a->Hkv * p.cblocks <= 65535 && p.per <= 2048 && a->H <= 65535 && a->n_tiles < 1 << 23 && (p.cols != MANY_COLS || (int64_t)a->n_tiles * a->Hkv * p.cblocks < 1 << 23), PCB_ERR_ARG,
+                "pcb_attn_pages: too many tiles, heads or tile rows (heads times tile rows up to 2^20, 2048 query heads a key head)");
+    PCB_REQUIRE((!p.groups && p.runs == 1) || (a->part && (uintptr_t)a->part % 16 == 0 && a->part_floats >= part_floats(p, a->Hkv, a->dim, a->n_tiles)), PCB_ERR_ARG,
+                "pcb_attn_pages: shared key runs need pcb_attn_pages_part floats");
     if (a->dtype == PCB_BF16)
         return a->code == PCB_CODE_E4M3 ? dispatch<bf16_t, PCB_CODE_E4M3>(*a, p, (hipStream_t)stream) : dispatch<bf16_t, PCB_CODE_INT8>(*a, p, (hipStream_t)stream);
     return a->code == PCB_CODE_E4M3 ? dispatch<float, PCB_CODE_E4M3>(*a, p, (hipStream_t)stream) : dispatch<float, PCB_CODE_INT8>(*a, p, (hipStream_t)stream);

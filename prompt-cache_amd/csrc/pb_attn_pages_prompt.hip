@@ -1,0 +1,297 @@
+// pcb_attn_pages for tiles of many columns (pb_attn_pages.hip: what a column, a step and a scale are): prompts behind cached prefixes, long questions.
+//
+// One workgroup = 128 columns of a tile and one key head, 32 a wave, over the keys they see (or a run of these, where the tiles are too few to fill the chip).  A step's 64 keys and
+// values become halves once for all four waves: codes go memory -> registers a step ahead, are converted and written to one of two LDS images while the other one is multiplied.
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_f16: a lane owns one column, its 32 scores of a step are its own operand of the second product (row 8 i + 4 h + j of the
+// first product's operand is key 16 (i / 2) + 8 h + 4 (i % 2) + j of 32, so lane half h holds keys 16 m + 8 h .. + 7), and a column's maximum is one exchange between two lanes.
+//
+// LDS rows are 16 bytes longer than their 64 DB halves of a key, or 64 keys of a value column: the sixteen lanes that are served at once fall on all banks.
+#include "pb_attn_pages.h"
+
+namespace {
+using namespace pcb;
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+// the larger, or the sum, of a lane's number and that of the lane 32 further
+__device__ __forceinline__ float max2(float v) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum2(float v) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+__device__ __forceinline__ float lane_of(float v, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)); }
+
+template <typename E, int CODE, int DB>
+__global__ __launch_bounds__(256, sizeof(E) == 2 && DB <= 2 ? 2 : 1) void attn_pages_prompt_kernel(pcb_attn_pages_args a, Plan pl) {
+    constexpr bool F32 = sizeof(E) == 4;
+    constexpr int PARTS = F32 ? 2 : 1, KK = 4 * DB, ND = 2 * DB;      // k-steps of 16 of the first product, row blocks of 32 of the second
+    constexpr int KLD = 64 * DB + 8, VLD = 72;
+    __shared__ __attribute__((aligned(16))) _Float16 Ks[2][64 * KLD], Vs[2][64 * DB * VLD];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, c = lane & 31;
+    const int hk = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, cb = rest % pl.cblocks, t = a.n_tiles - 1 - rest / pl.cblocks;   // (a prompt's last tiles, which see most keys, first)
+    const int dim = a.dim, ps = pl.ps, P = 1 << ps, per = pl.per;
+    Tile tl = tile_of(a, t, ps);
+    const int cols = tl.rows * per, col0 = cb * MANY_COLS;
+    if (col0 >= cols) return;
+    const int kv = tl.kv;
+    tl = rows_of(a, tl, row_of(pl, col0), row_of(pl, min(col0 + MANY_COLS, cols) - 1));
+    int s0 = tl.s0, s1 = tl.s1;
+    const bool split = pl.runs > 1 && s1 - s0 > pl.run;
+    if (split) {
+        s0 += (int)blockIdx.y * pl.run;
+        if ((int)blockIdx.y < pl.runs - 1) s1 = min(s1, s0 + pl.run);
+        if (s0 >= s1) return;
+    } else if (blockIdx.y > 0) {
+        return;
+    }
+    const int32_t* table = a.table + (int64_t)tl.seq * a.ld_table;
+    const int64_t plane = (int64_t)P * dim;
+    // pages and scales of sixteen steps at once: lane 4 i + k those of step i's keys 16 k ..
+    int pages = -1;
+    float kss = 1.0f, vss = 1.0f;
+    auto look = [&](int s) {
+        const int key = (s + (lane >> 2)) * 64 + 16 * (lane & 3);
+        pages = s + (lane >> 2) < s1 && key < kv ? table[key >> ps] : -1;
+        pages = pages >= 0 && pages < a.n_pages ? pages : -1;
+        const int64_t ph = (int64_t)(pages < 0 ? 0 : pages) * a.Hkv + hk;
+        kss = pages < 0 ? 1.0f : a.kscale[ph], vss = pages < 0 ? 1.0f : a.vscale[ph];
+    };
+    // staging: thread t takes 16-byte pieces t, t + 256, .. of the step's keys (4 DB a row) and of its value columns (four a column, the same sixteen keys each time)
+    const int vq = tid & 3;
+    u32x4 kr[DB], vr[DB];
+    auto fetch = [&](int s, int i) {
+#pragma unroll
+        for (int n = 0; n < DB; ++n) {
+            const int row = (n * 256 + tid) / (4 * DB), ch = tid % (4 * DB);
+            const int page = __shfl(pages, 4 * i + (row >> 4), 64);
+            const uint8_t* p = (const uint8_t*)a.kcodes + ((int64_t)(page < 0 ? 0 : page) * a.Hkv + hk) * plane + ((s * 64 + row) & (P - 1)) * dim;
+            kr[n] = *reinterpret_cast<const u32x4*>(p + 16 * min(ch, dim / 16 - 1));
+        }
+        const int page = __shfl(pages, 4 * i + vq, 64);
+        const uint8_t* p = (const uint8_t*)a.vcodes + ((int64_t)(page < 0 ? 0 : page) * a.Hkv + hk) * plane + ((s * 64 + 16 * vq) & (P - 1));
+#pragma unroll
+        for (int n = 0; n < DB; ++n) vr[n] = *reinterpret_cast<const u32x4*>(p + min(n * 64 + (tid >> 2), dim - 1) * P);
+        // values behind the last written key are whatever the memory held, and no number times 0 is 0 for all of them
+        const int have = page < 0 ? 0 : kv - (s * 64 + 16 * vq);
+        if (have < 16) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int k = have - 4 * e;
+                const uint32_t keep = k >= 4 ? 0xffffffffu : k <= 0 ? 0u : 0xffffffffu >> (32 - 8 * k);
+#pragma unroll
+                for (int n = 0; n < DB; ++n) vr[n][e] &= keep;
+            }
+        }
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int n = 0; n < DB; ++n) {
+            const int row = (n * 256 + tid) / (4 * DB), ch = tid % (4 * DB);
+            _Float16* k = &Ks[buf][row * KLD + 16 * ch];
+            *reinterpret_cast<h8*>(k) = half8<CODE>(u32x2{kr[n][0], kr[n][1]});
+            *reinterpret_cast<h8*>(k + 8) = half8<CODE>(u32x2{kr[n][2], kr[n][3]});
+            _Float16* v = &Vs[buf][(n * 64 + (tid >> 2)) * VLD + 16 * vq];
+            *reinterpret_cast<h8*>(v) = half8<CODE>(u32x2{vr[n][0], vr[n][1]});
+            *reinterpret_cast<h8*>(v + 8) = half8<CODE>(u32x2{vr[n][2], vr[n][3]});
+        }
+    };
+    int i = 0;
+    if (s0 < s1) {
+        look(s0);
+        fetch(s0, 0);
+    }
+    // this lane's column
+    const int col = col0 + 32 * wave + c;
+    const bool live = col < cols;
+    const int qr = live ? row_of(pl, col) : 0, h = hk * per + (live ? col - qr * per : 0), pos = live ? tl.pos + qr : -1;
+    const int lo = a.window > 0 ? pos - a.window + 1 : 0, hi = min(kv, pos + 1);
+    // keys that all, and that some of the wave's columns see
+    const int wc0 = col0 + 32 * wave, wc1 = min(wc0 + 32, cols) - 1;
+    const bool wave_live = wc0 < cols;
+    const int p0 = tl.pos + row_of(pl, wave_live ? wc0 : 0), p1 = tl.pos + row_of(pl, wave_live ? wc1 : 0);
+    const int all_lo = a.window > 0 ? p1 - a.window + 1 : 0, all_hi = wc0 + 32 <= cols ? min(kv, p0 + 1) : 0;
+    const int any_lo = a.window > 0 ? p0 - a.window + 1 : 0, any_hi = wave_live ? min(kv, p1 + 1) : 0;
+    h8 qf[PARTS][KK];
+    float qs;
+    {
+        const E* q = (const E*)a.q + ((int64_t)tl.row0 + qr) * a.ldq + (int64_t)h * a.q_head_stride;
+        float x[KK][8], m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KK; ++k) {
+            Frag<E> f;
+            zero8(f);
+            if (live && 16 * k < dim) f = load8(q + 16 * k + 8 * hh);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[k][e] = at8(f, e);
+                m = fmaxf(m, __builtin_fabsf(x[k][e]) < __builtin_inff() ? __builtin_fabsf(x[k][e]) : 0.0f);
+            }
+        }
+        // divided by a power of two, the row's largest element is 2^14 .. 2^15: what is 2^-28 of it is still a normal half
+        m = max2(m);
+        int e2 = (int)(__float_as_uint(m) >> 23) - 127 - 14;
+        e2 = e2 < -110 ? -110 : e2;
+        const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
+        qs = __uint_as_float((uint32_t)(127 + e2) << 23) * (F32 ? a.scale : a.scale * LOG2E);
+#pragma unroll
+        for (int k = 0; k < KK; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = x[k][e] * inv;
+                const _Float16 top = (_Float16)y;
+                qf[0][k][e] = top;
+                if constexpr (PARTS == 2) qf[1][k][e] = __builtin_fabsf(y) < __builtin_inff() ? (_Float16)(y - (float)top) : (_Float16)0.0f;
+            }
+    }
+    float M = NEG, l = 0.0f;
+    f16v o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+    if (s0 < s1) stage(0);
+    const int krow = (c >> 4) * 16 + ((c >> 2) & 1) * 8 + ((c >> 3) & 1) * 4 + (c & 3);   // the key of 32 that row c of the first product's operand is
+    int buf = 0;
+    for (int s = s0; s < s1; ++s) {
+        // the step's scales, before `look` takes the next ones' place
+        float ks[4], vs[4];
+        bool whole = s * 64 + 64 <= all_hi && s * 64 >= all_lo;
+        int page_ok = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            ks[q] = lane_of(kss, 4 * i + q), vs[q] = lane_of(vss, 4 * i + q);
+            page_ok |= (__builtin_amdgcn_readlane(pages, 4 * i + q) >= 0 ? 1 : 0) << q;
+        }
+        whole = whole && page_ok == 15;
+        const bool more = s + 1 < s1;
+        __syncthreads();                                              // the step's image is written, the other one read
+        i = (i + 1) & 15;
+        if (more) {
+            if (i == 0) look(s + 1);
+            fetch(s + 1, i);
+        }
+        if (s * 64 < any_hi && s * 64 + 64 > any_lo) {
+            f16v acc[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[b][e] = 0.0f;
+                const _Float16* k = &Ks[buf][(32 * b + krow) * KLD + 8 * hh];
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    const h8 f = *reinterpret_cast<const h8*>(k + 16 * kk);
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qf[p][kk], acc[b], 0, 0, 0);
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = s * 64 + 32 * b + 16 * (e >> 3) + 8 * hh + (e & 7);
+                        if (!(key >= lo && key < hi && (page_ok >> (2 * b + (e >> 3)) & 1))) acc[b][e] = NEG;
+                    }
+            }
+            float f[4], top = NEG;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                f[q] = qs * ks[q];
+                float m = acc[q >> 1][8 * (q & 1)];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) m = fmaxf(m, acc[q >> 1][8 * (q & 1) + e]);
+                top = fmaxf(top, m * f[q] + (F32 ? exp_of(vs[q]) * 0.693147181f : exp_of(vs[q])));
+            }
+            top = max2(top);
+            const float M_new = fmaxf(M, top), M_use = M_new == NEG ? 0.0f : M_new;
+            const float alpha = pow_of<E>(M - M_use);
+            h8 wf[PARTS][4];
+            float sum = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float part = 0.0f;
+                if constexpr (!F32) {
+                    const float off = exp_of(vs[q]) + 14.0f - M_use;  // vscale and 2^14 inside the exponent, out of the sum again
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[q >> 1][8 * (q & 1) + e], f[q], off));
+                        part += w;
+                        wf[0][q][e] = (_Float16)w;
+                    }
+                    sum = __builtin_fmaf(part, inv_pow2(vs[q]) * (1.0f / 16384.0f), sum);
+                } else {
+                    const float up = vs[q] * 16384.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float ex = exp_of_score(acc[q >> 1][8 * (q & 1) + e] * f[q], M_use), w = ex * up;
+                        part += ex;
+                        const _Float16 top16 = (_Float16)w;
+                        wf[0][q][e] = top16;
+                        wf[1][q][e] = (_Float16)(w - (float)top16);
+                    }
+                    sum += part;
+                }
+            }
+            l = l * alpha + sum;
+            if (!__all(M_new == M)) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+            }
+            M = M_new;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const _Float16* v = &Vs[buf][(32 * d + c) * VLD + 8 * hh];
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const h8 x = *reinterpret_cast<const h8*>(v + 16 * m);
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wf[p][m], o[d], 0, 0, 0);
+                }
+            }
+        }
+        if (more) stage(buf ^ 1);
+        buf ^= 1;
+    }
+    if (!live) return;
+    l = sum2(l);
+    E* op = (E*)a.out + ((int64_t)tl.row0 + qr) * a.ldo + (int64_t)h * a.out_head_stride;
+    const int cc = col - col0;
+    float* pp = a.part + ((((int64_t)t * a.Hkv + hk) * pl.cblocks + cb) * pl.runs + blockIdx.y) * MANY_COLS * (dim + 2);
+    const float f = split ? 1.0f : finished<E>(a, h, M, l, 16384.0f) * (1.0f / 16384.0f);
+    if (split && hh == 0) *reinterpret_cast<float2*>(pp + MANY_COLS * dim + 2 * cc) = float2{M, l};
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int at = 32 * d + 8 * q + 4 * hh;
+            if (at >= dim) continue;
+            if (split)
+                *reinterpret_cast<f4*>(pp + cc * dim + at) = f4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+            else
+                store4(op + at, o[d][4 * q] * f, o[d][4 * q + 1] * f, o[d][4 * q + 2] * f, o[d][4 * q + 3] * f);
+        }
+}
+
+template <typename E, int CODE>
+int launch(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
+    const dim3 grid((unsigned)((int64_t)a.n_tiles * a.Hkv * pl.cblocks), pl.runs), block(256);
+    if (a.dim <= 64)
+        hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 1>), grid, block, 0, stream, a, pl);
+    else if (a.dim <= 128)
+        hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 2>), grid, block, 0, stream, a, pl);
+    else
+        hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 4>), grid, block, 0, stream, a, pl);
+    return pcb_check_launch("attn_pages_prompt_kernel");
+}
+
+}  // namespace
+
+int pcb_attn_pages_prompt(const pcb_attn_pages_args& a, const pcb::Plan& pl, hipStream_t stream) {
+    if (a.dtype == PCB_BF16) return a.code == PCB_CODE_E4M3 ? launch<pcb::bf16_t, PCB_CODE_E4M3>(a, pl, stream) : launch<pcb::bf16_t, PCB_CODE_INT8>(a, pl, stream);
+    return a.code == PCB_CODE_E4M3 ? launch<float, PCB_CODE_E4M3>(a, pl, stream) : launch<float, PCB_CODE_INT8>(a, pl, stream);
+}

@@ -1184,39 +1184,53 @@ def rec_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lds_, reqs: torc
 
 
 # ---- keys and values in 8 bits, in pages ------------------------------------------------------------------------------------------------------
-def _flat(t: Optional[torch.Tensor], dtype, numel: int, what: str) -> None:
-    """``t`` (optional) holds at least ``numel`` elements of ``dtype`` one after the other on the current device."""
+def _flat(t: Optional[torch.Tensor], dtype, numel: int, dev: int, what: str) -> Optional[int]:
+    """The address of ``t`` (optional), which holds at least ``numel`` elements of ``dtype`` one after the other on device ``dev``."""
     if t is None:
-        return
-    _want(t, dtype, what)
-    if t.numel() < numel:
-        raise ValueError(f"{what}: {numel} elements are needed, got {t.numel()}")
-    _here(t, what)
+        return None
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous() or t.numel() < numel:
+        if t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
+            _want(t, dtype, what)
+        raise ValueError(f"{what}: {numel} elements on cuda:{dev} are needed, got {t.numel()} on {t.device}")
+    return t.data_ptr()
 
 
-def _here(t: torch.Tensor, what: str) -> None:
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+def _device_of(t: torch.Tensor, what: str) -> int:
+    """The device that ``t`` lies on, which has to be the current one (its stream is the one a call goes to)."""
+    dev = t.get_device()
+    if dev < 0:
+        raise TypeError(f"{what}: need a device tensor, got one on {t.device}")
+    if dev != torch.cuda.current_device():
         raise ValueError(f"{what} lies on {t.device}, and the current device is cuda:{torch.cuda.current_device()}")
+    return dev
 
 
-def _pool(kcodes: torch.Tensor, kscale: torch.Tensor, vcodes: torch.Tensor, vscale: torch.Tensor, what: str):
-    """Checks a pool: codes ``[pages, Hkv, P, dim]`` / ``[pages, Hkv, dim, P]``, scales ``[pages, Hkv]``; -> (code, pages, P, Hkv, dim)."""
-    if kcodes.dtype not in CODES or vcodes.dtype != kcodes.dtype:
+def _pool(kcodes: torch.Tensor, kscale: torch.Tensor, vcodes: torch.Tensor, vscale: torch.Tensor, dev: int, what: str):
+    """Checks a pool: codes ``[pages, Hkv, P, dim]`` / ``[pages, Hkv, dim, P]``, scales ``[pages, Hkv]``; -> (code, its pointers, (pages, P), (Hkv, dim))."""
+    code = CODES.get(kcodes.dtype)
+    if code is None or vcodes.dtype is not kcodes.dtype:
         raise TypeError(f"{what}: codes are both float8_e4m3fn or both int8, got {kcodes.dtype} and {vcodes.dtype}")
     if kcodes.dim() != 4 or vcodes.shape != (kcodes.shape[0], kcodes.shape[1], kcodes.shape[3], kcodes.shape[2]):
         raise ValueError(f"{what}: key codes [pages, heads, P, dim] and value codes [pages, heads, dim, P], got {tuple(kcodes.shape)} and {tuple(vcodes.shape)}")
     pages, Hkv, P, dim = kcodes.shape
-    _flat(kcodes, kcodes.dtype, 0, f"{what} key codes"); _flat(vcodes, kcodes.dtype, 0, f"{what} value codes")
-    _flat(kscale, torch.float32, pages * Hkv, f"{what} key scales"); _flat(vscale, torch.float32, pages * Hkv, f"{what} value scales")
-    return CODES[kcodes.dtype], pages, P, Hkv, dim
+    ptrs = (_flat(kcodes, kcodes.dtype, 0, dev, "key codes of " + what), _flat(kscale, torch.float32, pages * Hkv, dev, "key scales of " + what),
+            _flat(vcodes, kcodes.dtype, 0, dev, "value codes of " + what), _flat(vscale, torch.float32, pages * Hkv, dev, "value scales of " + what))
+    return code, ptrs, (pages, P), (Hkv, dim)
 
 
-def _heads(t: torch.Tensor, heads: int, dim: int, what: str):
-    """Rows ``[rows, heads, dim]`` with neighbouring elements of a head; -> (row stride, head stride)."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or (t.stride(2) != 1 and t.numel() > 0):
-        raise ValueError(f"{what}: rows [rows, {heads}, {dim}] whose last axis is contiguous, got {tuple(t.shape)} with strides {t.stride()}")
-    _here(t, what)
-    return t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if heads > 1 else 0
+def _heads(t: torch.Tensor, heads: int, dim: int, dev: int, what: str):
+    """Rows ``[rows, heads, dim]`` with neighbouring elements of a head; -> (address, row stride, head stride)."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or stride[2] != 1 and t.numel() > 0 or t.get_device() != dev:
+        raise ValueError(f"{what}: rows [rows, {heads}, {dim}] on cuda:{dev} whose last axis is contiguous, got {tuple(shape)} with strides {stride} on {t.device}")
+    return t.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1] if heads > 1 else 0
+
+
+def _table(table: torch.Tensor, n: int, dev: int, what: str):
+    """An int32 block table of at least ``n`` contiguous rows; -> (address, row stride, pages)."""
+    if table.dim() != 2 or table.shape[0] < n or table.dtype is not torch.int32 or table.stride(1) != 1 and table.numel() > 0 or table.get_device() != dev:
+        raise ValueError(f"{what}: a table int32 [{n}, pages] on cuda:{dev} with contiguous rows, got {table.dtype} {tuple(table.shape)} on {table.device}")
+    return table.data_ptr(), max(table.stride(0), table.shape[1]) if table.shape[0] < 2 else table.stride(0), table.shape[1]
 
 
 def page_tables(cached: torch.Tensor, brings: torch.Tensor, table: torch.Tensor, page_size: int, *, row_slot: torch.Tensor, kv_len=None, row_start=None, row_seq=None,
@@ -1225,29 +1239,27 @@ def page_tables(cached: torch.Tensor, brings: torch.Tensor, table: torch.Tensor,
     and brings (below zero: it is over); ``table`` int32 [n, max_pages] gets the pages taken from ``ring`` (int32, the free pages; ``ring_state`` int32 [2 or
     more] {first, number}; ``ring_out`` int32 [4], may be ``ring_state``).  ``row_slot`` int64 [rows] and, optional, ``row_seq`` / ``row_pos`` int32 [rows],
     ``row_start`` [n + 1], ``kv_len`` [n], ``tiles`` [n + rows // tile_rows, 4], ``status`` [2] are written; without ``ring`` the table holds all pages already."""
-    n, rows = cached.numel(), row_slot.numel()
-    if table.dim() != 2 or table.shape[0] < n or table.dtype != torch.int32 or table.stride(1) != 1 or table.stride(0) < table.shape[1]:
-        raise ValueError(f"page_tables table: int32 [{n}, pages] with contiguous rows, got {table.dtype} {tuple(table.shape)}")
-    _here(table, "page_tables table")
-    for t, dtype, numel, what in ((cached, torch.int32, n, "cached"), (brings, torch.int32, n, "brings"), (keep, torch.int32, n, "keep"), (kv_len, torch.int32, n, "kv_len"),
-                                  (row_start, torch.int32, n + 1, "row_start"), (row_seq, torch.int32, rows, "row_seq"), (row_pos, torch.int32, rows, "row_pos"),
-                                  (row_slot, torch.int64, rows, "row_slot"), (status, torch.int32, 2, "status"), (ring, torch.int32, 1, "ring"),
-                                  (ring_state, torch.int32, 2, "ring_state"), (ring_out, torch.int32, 4, "ring_out"), (tiles, torch.int32, 0, "tiles")):
-        _flat(t, dtype, numel, "page_tables " + what)
-    a = PageTablesArgs(C.sizeof(PageTablesArgs), n, table.shape[1], table.stride(0), page_size, _p(cached), _p(brings), _p(keep), _p(table),
-                       _p(ring), 0 if ring is None else ring.numel(), _p(ring_state), _p(ring_out), _p(kv_len), _p(row_start), _p(row_seq), _p(row_pos), _p(row_slot), rows,
-                       _p(tiles), 0 if tiles is None else tiles.numel() // 4, tile_rows, _p(status))
+    n, rows, i32 = cached.numel(), row_slot.numel(), torch.int32
+    dev = _device_of(cached, "page_tables cached")
+    tab, ld, pages = _table(table, n, dev, "page_tables")
+    a = PageTablesArgs(C.sizeof(PageTablesArgs), n, pages, ld, page_size, _flat(cached, i32, n, dev, "cached"), _flat(brings, i32, n, dev, "brings"),
+                       _flat(keep, i32, n, dev, "keep"), tab, _flat(ring, i32, 1, dev, "ring"), 0 if ring is None else ring.numel(),
+                       _flat(ring_state, i32, 2, dev, "ring_state"), _flat(ring_out, i32, 4, dev, "ring_out"), _flat(kv_len, i32, n, dev, "kv_len"),
+                       _flat(row_start, i32, n + 1, dev, "row_start"), _flat(row_seq, i32, rows, dev, "row_seq"), _flat(row_pos, i32, rows, dev, "row_pos"),
+                       _flat(row_slot, torch.int64, rows, dev, "row_slot"), rows, _flat(tiles, i32, 0, dev, "tiles"), 0 if tiles is None else tiles.numel() // 4, tile_rows,
+                       _flat(status, i32, 2, dev, "status"))
     check(load().pcb_page_tables(C.byref(a), _stream()), "pcb_page_tables")
 
 
 def _pages_rows(name: str, k, v, row_slot, kcodes, kscale, vcodes, vscale) -> None:
-    code, pages, P, Hkv, dim = _pool(kcodes, kscale, vcodes, vscale, name)
-    if k.dtype != v.dtype or k.shape != v.shape:
+    code, ptrs, (pages, P), (Hkv, dim) = _pool(kcodes, kscale, vcodes, vscale, k.get_device(), name)
+    dev = _device_of(k, name)
+    if k.dtype is not v.dtype or k.shape != v.shape:
         raise TypeError(f"{name}: keys and values of one type and shape, got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
-    _flat(row_slot, torch.int64, k.shape[0], f"{name} row_slot")
-    a = PagesRowsArgs(C.sizeof(PagesRowsArgs), _code(k), code, _p(k), *_heads(k, Hkv, dim, f"{name} keys"), _p(v), *_heads(v, Hkv, dim, f"{name} values"), _p(row_slot),
-                      k.shape[0], _p(kcodes), _p(kscale), _p(vcodes), _p(vscale), pages, P, Hkv, dim)
-    check(getattr(load(), "pcb_" + name)(C.byref(a), _stream()), "pcb_" + name)
+    rows = k.shape[0]
+    a = PagesRowsArgs(C.sizeof(PagesRowsArgs), _code(k), code, *_heads(k, Hkv, dim, dev, name), *_heads(v, Hkv, dim, dev, name),
+                      _flat(row_slot, torch.int64, rows, dev, "row_slot of " + name), rows, *ptrs, pages, P, Hkv, dim)
+    check(getattr(load(), "pcb_" + name)(C.byref(a), _stream()), name)
 
 
 def pages_append(k: torch.Tensor, v: torch.Tensor, row_slot: torch.Tensor, kcodes: torch.Tensor, kscale: torch.Tensor, vcodes: torch.Tensor, vscale: torch.Tensor) -> None:
@@ -1274,22 +1286,19 @@ def attn_pages(q: torch.Tensor, tiles: torch.Tensor, tile_rows: int, kv_len: tor
     """Causal attention of rows ``q`` [rows, H, dim] over the pages of ``table`` int32 [n, max_pages], ``kv_len`` int32 [n] tokens of which are written; ``tiles`` int32
     [t, 4] {sequence, first position, rows, first flat row} as ``page_tables`` makes them, of at most ``tile_rows`` rows; ``sink`` fp32 [H].  ``longest``: an upper bound
     of ``kv_len`` known to the host (0: the table's width); ``part`` fp32 of ``attn_pages_part(...)`` floats (None: allocated when it is needed)."""
-    code, pages, P, Hkv, dim = _pool(kcodes, kscale, vcodes, vscale, "attn_pages")
-    if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype or q.shape[1] % Hkv:
+    code, ptrs, (pages, P), (Hkv, dim) = _pool(kcodes, kscale, vcodes, vscale, q.get_device(), "attn_pages")
+    dev = _device_of(q, "attn_pages queries")
+    if q.dim() != 3 or out.shape != q.shape or out.dtype is not q.dtype or q.shape[1] % Hkv:
         raise ValueError(f"attn_pages: queries and results [rows, H, {dim}], H a multiple of {Hkv}, of one type; got {q.dtype} {tuple(q.shape)} and {out.dtype} {tuple(out.shape)}")
     rows, H = q.shape[0], q.shape[1]
-    n = kv_len.numel()
-    if table.dim() != 2 or table.shape[0] < n or table.dtype != torch.int32 or table.stride(1) != 1:
-        raise ValueError(f"attn_pages table: int32 [{n}, pages] with contiguous rows, got {table.dtype} {tuple(table.shape)}")
-    _here(table, "attn_pages table")
-    _flat(tiles, torch.int32, 0, "attn_pages tiles"); _flat(kv_len, torch.int32, 0, "attn_pages kv_len")
-    _flat(sink, torch.float32, H, "attn_pages sink"); _flat(part, torch.float32, 0, "attn_pages part")
-    longest = longest if longest > 0 else table.shape[1] * P
-    n_tiles = tiles.numel() // 4
+    n, n_tiles = kv_len.numel(), tiles.numel() // 4
+    tab, ld, wide = _table(table, n, dev, "attn_pages")
+    longest = longest if longest > 0 else wide * P
     if part is None:
         floats = attn_pages_part(rows, H, Hkv, dim, n_tiles, tile_rows, longest)
         part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    a = AttnPagesArgs(C.sizeof(AttnPagesArgs), _code(q), code, _p(q), *_heads(q, H, dim, "attn_pages queries"), _p(tiles), n_tiles, tile_rows, rows, _p(kv_len), _p(table),
-                      table.stride(0), n, table.shape[1], _p(kcodes), _p(kscale), _p(vcodes), _p(vscale), pages, P, H, Hkv, dim, float(scale), int(window), _p(sink),
-                      _p(out), *_heads(out, H, dim, "attn_pages results"), longest, _p(part), 0 if part is None else part.numel())
+    a = AttnPagesArgs(C.sizeof(AttnPagesArgs), _code(q), code, *_heads(q, H, dim, dev, "attn_pages queries"), _flat(tiles, torch.int32, 0, dev, "attn_pages tiles"), n_tiles,
+                      tile_rows, rows, _flat(kv_len, torch.int32, 0, dev, "attn_pages kv_len"), tab, ld, n, wide, *ptrs, pages, P, H, Hkv, dim, float(scale), int(window),
+                      _flat(sink, torch.float32, H, dev, "attn_pages sink"), *_heads(out, H, dim, dev, "attn_pages results"), longest,
+                      _flat(part, torch.float32, 0, dev, "attn_pages part"), 0 if part is None else part.numel())
     check(load().pcb_attn_pages(C.byref(a), _stream()), "pcb_attn_pages")
