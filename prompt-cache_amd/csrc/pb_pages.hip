@@ -173,25 +173,47 @@ __global__ __launch_bounds__(NT) void page_tables_kernel(pcb_page_tables_args a,
 }
 
 // ---- rows into pages ------------------------------------------------------------------------------------------------------------------------
-// eight neighbouring elements as floats
-__device__ __forceinline__ void row8(const bf16_t* p, float (&o)[8]) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+// sixteen bytes of a row, CE elements
+template <typename E>
+struct Piece {
+    static constexpr int CE = 16 / sizeof(E);
+    u32x4 w;
+    __device__ __forceinline__ float at(int e) const {
+        if constexpr (sizeof(E) == 2)
+            return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+        else
+            return __uint_as_float(w[e]);
+    }
+};
+// the largest magnitude's bits among what `m` holds (bf16: pairs) and a piece: numbers order as their bits do, and what is no finite number comes out above them
+__device__ __forceinline__ uint32_t larger(uint32_t m, const Piece<bf16_t>& p) {
+    typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+    u2 r = __builtin_bit_cast(u2, m);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[2 * e] = __uint_as_float(w[e] << 16), o[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    for (int q = 0; q < 4; ++q) r = __builtin_elementwise_max(r, __builtin_bit_cast(u2, p.w[q] & 0x7fff7fffu));
+    return __builtin_bit_cast(uint32_t, r);
 }
-__device__ __forceinline__ void row8(const float* p, float (&o)[8]) {
-    const f4 a = *reinterpret_cast<const f4*>(p), b = *reinterpret_cast<const f4*>(p + 4);
+__device__ __forceinline__ uint32_t larger(uint32_t m, const Piece<float>& p) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = a[e], o[4 + e] = b[e];
+    for (int q = 0; q < 4; ++q) m = max(m, p.w[q] & 0x7fffffffu);
+    return m;
 }
-__device__ __forceinline__ void put8(bf16_t* p, const float (&o)[8]) {
-    *reinterpret_cast<u32x4*>(p) = u32x4{bf16_pair(o[0], o[1]), bf16_pair(o[2], o[3]), bf16_pair(o[4], o[5]), bf16_pair(o[6], o[7])};
-}
-__device__ __forceinline__ void put8(float* p, const float (&o)[8]) {
-    *reinterpret_cast<f4*>(p) = f4{o[0], o[1], o[2], o[3]};
-    *reinterpret_cast<f4*>(p + 4) = f4{o[4], o[5], o[6], o[7]};
-}
+template <typename E>
+__device__ __forceinline__ float largest(uint32_t m) { return __uint_as_float(sizeof(E) == 2 ? max(m & 0xffff0000u, m << 16) : m); }
 __device__ __forceinline__ float size_of(float x) { return __builtin_fabsf(x) < __builtin_inff() ? __builtin_fabsf(x) : 0.0f; }
+
+// four numbers within the codes' range, in units of 1 / inv, as codes.  int8: added to 1.5 2^23 a number is rounded to a whole one, which the last byte then is
+template <int CODE>
+__device__ __forceinline__ uint32_t codes_of(float a, float b, float c, float d, float inv) {
+    if (CODE == PCB_CODE_E4M3) {
+        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, lo, true);
+    }
+    const float big = 12582912.0f;
+    const uint32_t x = __builtin_amdgcn_perm(__float_as_uint(__builtin_fmaf(b, inv, big)), __float_as_uint(__builtin_fmaf(a, inv, big)), 0x0c0c0400u);
+    const uint32_t y = __builtin_amdgcn_perm(__float_as_uint(__builtin_fmaf(d, inv, big)), __float_as_uint(__builtin_fmaf(c, inv, big)), 0x0c0c0400u);
+    return x | y << 16;
+}
 
 // four codes anew, in units that are 1 / ratio times as large
 template <int CODE>
@@ -200,6 +222,8 @@ __device__ __forceinline__ uint32_t again(uint32_t w, float ratio) {
     from_codes<CODE>(w, o);
     return to_codes<CODE>(o[0] * ratio, o[1] * ratio, o[2] * ratio, o[3] * ratio);
 }
+// the bytes k .. 3 of a word
+__device__ __forceinline__ uint32_t from_byte(int k) { return k >= 4 ? 0u : k <= 0 ? 0xffffffffu : 0xffffffffu << (8 * k); }
 
 struct RowsView {
     const int64_t* slot;
@@ -212,93 +236,116 @@ struct RowsView {
     }
 };
 
-// One wave: the rows r0 .. r0 + n - 1 (n <= P), all of one page, their first slot s0; `even`: their slots follow one another.
+// One wave: the rows r0 .. r0 + n - 1 (n <= P), all of one page, their first slot s0, their smallest place off_min; `even`: their slots follow one another.
+//
+// A lane takes sixteen rows, those whose places share a multiple of 16, and sixteen bytes of each: the maximum, a key row's codes and a value column's sixteen codes (one
+// store) all come out of the same registers, and a page of 64 rows of 128 bf16 elements is one such load for the wave, read once.  (Rows first for the maximum, then again for
+// the codes, value columns a row a lane at a time: 55 us for 28 600 rows of 8 heads.)  Larger pages are read twice, the second time from the caches.
 template <typename E, int CODE, bool VALUES>
 __device__ void append_run(const pcb_pages_rows_args& a, const RowsView& v, int64_t r0, int n, int64_t s0, int off_min, bool even, int h, int lane) {
-    const int P = 1 << v.ps, dim = a.dim, cpr = dim / 8;
+    constexpr int CE = Piece<E>::CE;
+    const int P = 1 << v.ps, dim = a.dim, cpr = dim / CE;             // pieces of a row
     const int64_t page = s0 >> v.ps;
-    const E* src = (const E*)(VALUES ? a.v : a.k) + (int64_t)h * (VALUES ? a.v_head_stride : a.k_head_stride);
     const int64_t ld = VALUES ? a.ldv : a.ldk;
+    const E* src = (const E*)(VALUES ? a.v : a.k) + (int64_t)h * (VALUES ? a.v_head_stride : a.k_head_stride) + r0 * ld;
     float* scale = (VALUES ? a.vscale : a.kscale) + page * a.Hkv + h;
     uint8_t* codes = (uint8_t*)(VALUES ? a.vcodes : a.kcodes) + (page * a.Hkv + h) * (int64_t)P * dim;
-    const int chunks = n * cpr;
-    float m = 0.0f;
-#pragma unroll 4
-    for (int i = lane; i < chunks; i += 64) {
-        const int r = i / cpr, c = i - r * cpr;
-        float x[8];
-        row8(src + (r0 + r) * ld + c * 8, x);
+    const float was = off_min > 0 ? *scale : 0.0f;                    // (asked for beside the rows)
+    const int off0 = even ? (int)(s0 & (P - 1)) : 0, g0 = off0 >> 4;  // (rows in another order: sixteen as they come)
+    const int tasks = (((off0 + n - 1) >> 4) - g0 + 1) * cpr;
+    Piece<E> x[16];
+    int f = 0, c = 0;                                                 // the lane's rows f .. f + 15, of which those in 0 .. n - 1 exist (the others repeat one), and its piece
+    auto load = [&](int i) {
+        const int grp = i / cpr;
+        f = 16 * (g0 + grp) - off0, c = i - grp * cpr;
+        const E* p = src + c * CE;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmaxf(m, size_of(x[e]));
+        for (int k = 0; k < 16; ++k) x[k].w = *reinterpret_cast<const u32x4*>(p + min(max(f + k, 0), n - 1) * ld);
+    };
+    uint32_t mb = 0;
+    for (int i = lane; i < tasks; i += 64) {
+        load(i);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) mb = larger(mb, x[k]);
     }
-    float s = scale_for<CODE>(wave_max(m));
-    if (off_min > 0) {
-        const float old = *scale;
-        if (old >= s) {
-            s = old;
+    float m = wave_max(largest<E>(mb));                               // (as numbers: a NaN among them is passed over ..)
+    const bool odd = __any(!(largest<E>(mb) <= code_top<CODE>() * 1099511627776.0f));   // .. but seen here; as are infinities, and numbers beyond the largest scale's range
+    if (odd) {
+        m = 0.0f;
+        for (int i = lane; i < n * cpr; i += 64) {
+            Piece<E> y;
+            y.w = *reinterpret_cast<const u32x4*>(src + i / cpr * ld + i % cpr * CE);
+#pragma unroll
+            for (int e = 0; e < CE; ++e) m = fmaxf(m, size_of(y.at(e)));
+        }
+        m = wave_max(m);
+    }
+    float s = scale_for<CODE>(m);
+    if (was >= s) {
+        s = was;
+    } else if (off_min > 0) {
+        // the codes in front of the first new row, in the new units.  (An old scale of a page that this library wrote is a power of two.)
+        const float ratio = was * inv_pow2(s);
+        if (!VALUES) {
+            uint32_t* w = (uint32_t*)codes;
+            for (int i = lane; i < off_min * dim / 4; i += 64) w[i] = again<CODE>(w[i], ratio);
         } else {
-            // the codes in front of the first new row, in the new units.  (An old scale of a page that this library wrote is a power of two.)
-            const float ratio = old * inv_pow2(s);
-            if (!VALUES) {
-                uint32_t* w = (uint32_t*)codes;
-                for (int i = lane; i < off_min * dim / 4; i += 64) w[i] = again<CODE>(w[i], ratio);
-            } else {
-                const int words = (off_min + 3) / 4;
-                for (int i = lane; i < words * dim; i += 64) {
-                    const int d = i / words, k = i - d * words;
-                    uint32_t* w = (uint32_t*)(codes + (int64_t)d * P) + k;
-                    const uint32_t was = *w, now = again<CODE>(was, ratio);
-                    const int left = off_min - 4 * k;                 // bytes of the word that are in front of the first new row
-                    const uint32_t keep = left >= 4 ? 0u : 0xffffffffu << (8 * left);
-                    *w = (now & ~keep) | (was & keep);
-                }
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (other lanes write the rest of these words)
+            const int words = (off_min + 3) / 4;
+            for (int i = lane; i < words * dim; i += 64) {
+                const int d = i / words, k = i - d * words;
+                uint32_t* w = (uint32_t*)(codes + (int64_t)d * P) + k;
+                const uint32_t old = *w, now = again<CODE>(old, ratio), keep = from_byte(off_min - 4 * k);
+                *w = (now & ~keep) | (old & keep);
             }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // (other lanes take up the rest of these words)
         }
     }
     if (lane == 0) *scale = s;
     const float inv = inv_pow2(s);
-    if (!VALUES) {
-#pragma unroll 4
-        for (int i = lane; i < chunks; i += 64) {
-            const int r = i / cpr, c = i - r * cpr;
-            const int off = even ? (int)(s0 & (P - 1)) + r : (int)(v.at(r0 + r) & (P - 1));
-            float x[8];
-            row8(src + (r0 + r) * ld + c * 8, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= inv;
-            *reinterpret_cast<u32x2*>(codes + (int64_t)off * dim + c * 8) =
-                u32x2{to_codes<CODE>(x[0], x[1], x[2], x[3]), to_codes<CODE>(x[4], x[5], x[6], x[7])};
+    if (odd || !even) {                                               // element by element
+        for (int i = lane; i < n * dim; i += 64) {
+            const int r = i / dim, d = i - r * dim, off = (int)(v.at(r0 + r) & (P - 1));
+            const uint8_t code = (uint8_t)to_codes<CODE>(to_f32(src[r * ld + d]) * inv, 0.f, 0.f, 0.f);
+            codes[VALUES ? (int64_t)d * P + off : (int64_t)off * dim + d] = code;
         }
         return;
     }
-    // values: a lane takes a column; sixteen rows that fill a 16-byte piece of it go out at once
-    const int off0 = (int)(s0 & (P - 1));
-    for (int d0 = 0; d0 < dim; d0 += 64) {
-        const int d = d0 + lane;
-        if (d >= dim) break;
-        uint8_t* col = codes + (int64_t)d * P;
-        int r = 0;
-        while (r < n) {
-            if (even && (off0 + r) % 16 == 0 && n - r >= 16) {
-                float x[16];
+    for (int i = lane; i < tasks; i += 64) {
+        if (tasks > 64) load(i);
+        const int lo = max(0, -f), hi = min(16, n - f);               // the lane's rows that exist
+        if (!VALUES) {
+            uint8_t* dst = codes + (int64_t)(off0 + f) * dim + c * CE;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = to_f32(src[(r0 + r + e) * ld + d]) * inv;
-                u32x4 w;
+            for (int k = 0; k < 16; ++k) {
+                uint32_t w[CE / 4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = to_codes<CODE>(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-                *reinterpret_cast<u32x4*>(col + off0 + r) = w;
-                r += 16;
-            } else {
-                const int off = even ? off0 + r : (int)(v.at(r0 + r) & (P - 1));
-                col[off] = (uint8_t)(to_codes<CODE>(to_f32(src[(r0 + r) * ld + d]) * inv, 0.f, 0.f, 0.f) & 255u);
-                ++r;
+                for (int q = 0; q < CE / 4; ++q) w[q] = codes_of<CODE>(x[k].at(4 * q), x[k].at(4 * q + 1), x[k].at(4 * q + 2), x[k].at(4 * q + 3), inv);
+                if (k < lo || k >= hi) continue;
+                if constexpr (CE == 8)
+                    *reinterpret_cast<u32x2*>(dst + k * dim) = u32x2{w[0], w[1]};
+                else
+                    *reinterpret_cast<uint32_t*>(dst + k * dim) = w[0];
             }
+            continue;
+        }
+        u32x4* dst = reinterpret_cast<u32x4*>(codes + (int64_t)(c * CE) * P + off0 + f);
+        const int step = P / 16;
+        u32x4 keep;                                                   // what of the columns' pieces stays
+#pragma unroll
+        for (int q = 0; q < 4; ++q) keep[q] = ~from_byte(lo - 4 * q) | from_byte(hi - 4 * q);
+        const bool some = lo > 0 || hi < 16;
+#pragma unroll
+        for (int e = 0; e < CE; ++e) {
+            u32x4 w;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) w[q] = codes_of<CODE>(x[4 * q].at(e), x[4 * q + 1].at(e), x[4 * q + 2].at(e), x[4 * q + 3].at(e), inv);
+            if (some) w = (w & ~keep) | (dst[e * step] & keep);
+            dst[e * step] = w;
         }
     }
 }
 
-// blockIdx.y: keys or values.  A wave looks at WIN rows of one head and takes the runs that start there.
+// blockIdx.y: keys or values.  A wave looks at `win` rows of one head and takes the runs that start there.
 template <typename E, int CODE>
 __global__ __launch_bounds__(256) void pages_append_kernel(pcb_pages_rows_args a, RowsView v, int win) {
     const int lane = threadIdx.x & 63;
@@ -337,65 +384,78 @@ __global__ __launch_bounds__(256) void pages_append_kernel(pcb_pages_rows_args a
 }
 
 // ---- rows out of pages ------------------------------------------------------------------------------------------------------------------------
-// A wave takes, of one head, the groups of rows that start in its window: neighbours whose slots follow one another within 16 slots from a multiple of 16.
+// eight neighbouring elements of a row
+__device__ __forceinline__ void put8(bf16_t* p, const float (&o)[8]) {
+    *reinterpret_cast<u32x4*>(p) = u32x4{bf16_pair(o[0], o[1]), bf16_pair(o[2], o[3]), bf16_pair(o[4], o[5]), bf16_pair(o[6], o[7])};
+}
+__device__ __forceinline__ void put8(float* p, const float (&o)[8]) {
+    *reinterpret_cast<f4*>(p) = f4{o[0], o[1], o[2], o[3]};
+    *reinterpret_cast<f4*>(p + 4) = f4{o[4], o[5], o[6], o[7]};
+}
+
+// A wave takes `win` rows of one head, keys or values.  Keys: a lane eight codes of a row.  Values: rows whose slots follow one another within sixteen are a group, and a lane takes
+// eight columns of one, sixteen codes each, and stores eight elements a row.
 template <typename E, int CODE>
-__global__ __launch_bounds__(256) void pages_read_kernel(pcb_pages_rows_args a, RowsView v) {
-    constexpr int WIN = 16;
-    const int lane = threadIdx.x & 63, dim = a.dim, P = 1 << v.ps;
+__global__ __launch_bounds__(256) void pages_read_kernel(pcb_pages_rows_args a, RowsView v, int win) {
+    const int lane = threadIdx.x & 63, dim = a.dim, P = 1 << v.ps, cpr = dim / 8;
     const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int h = (int)(unit % a.Hkv);
-    const int64_t w0 = unit / a.Hkv * WIN;
+    const int64_t w0 = unit / a.Hkv * win;
     if (w0 >= a.n_rows) return;
+    const int64_t mine = lane < win ? v.at(w0 + lane) : -1;
     if (blockIdx.y == 0) {
-        const int cpr = dim / 16;
-        for (int i = lane; i < WIN * cpr; i += 64) {
+        for (int i = lane; i - lane < win * cpr; i += 64) {
             const int r = i / cpr, c = i - r * cpr;
-            const int64_t s = v.at(w0 + r);
-            if (s < 0) continue;
+            const int64_t s = __shfl(mine, r < win ? r : 0, 64);
+            if (r >= win || s < 0) continue;
             const int64_t page = s >> v.ps;
-            const u32x4 w = *reinterpret_cast<const u32x4*>((const uint8_t*)a.kcodes + ((page * a.Hkv + h) * P + (s & (P - 1))) * dim + c * 16);
+            const u32x2 w = *reinterpret_cast<const u32x2*>((const uint8_t*)a.kcodes + ((page * a.Hkv + h) * P + (s & (P - 1))) * dim + c * 8);
             const float sc = a.kscale[page * a.Hkv + h];
-            E* dst = (E*)a.k + (w0 + r) * a.ldk + (int64_t)h * a.k_head_stride + c * 16;
+            float o[8];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float o[8];
+            for (int q = 0; q < 2; ++q) {
+                float x[4];
+                from_codes<CODE>(w[q], x);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float x[4];
-                    from_codes<CODE>(w[2 * half + e], x);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[4 * e + j] = x[j] * sc;
-                }
-                put8(dst + 8 * half, o);
+                for (int j = 0; j < 4; ++j) o[4 * q + j] = x[j] * sc;
             }
+            put8((E*)a.k + (w0 + r) * a.ldk + (int64_t)h * a.k_head_stride + c * 8, o);
         }
         return;
     }
-    const int64_t mine = lane < WIN ? v.at(w0 + lane) : -1, prev = lane < WIN ? v.at(w0 + lane - 1) : -1;
-    uint64_t starts = __ballot(mine >= 0 && (prev < 0 || prev + 1 != mine || mine % 16 == 0));
-    while (starts) {
-        const int i = __builtin_ctzll(starts);
-        starts &= starts - 1;
-        const int64_t r0 = w0 + i, s0 = __shfl(mine, i, 64), page = s0 >> v.ps;
-        const int most = 16 - (int)(s0 & 15);
-        const int64_t s = lane < most ? v.at(r0 + lane) : -1;
-        const uint64_t in = __ballot(s >= 0 && s == s0 + lane);
-        const int n = ~in ? __builtin_ctzll(~in) : 64;
-        const float sc = a.vscale[page * a.Hkv + h];
-        const uint8_t* codes = (const uint8_t*)a.vcodes + (page * a.Hkv + h) * (int64_t)P * dim + (s0 & (P - 1) & ~15);
-        E* dst = (E*)a.v + r0 * a.ldv + (int64_t)h * a.v_head_stride;
+    const int64_t prev = __shfl_up(mine, 1, 64);
+    const uint64_t there = __ballot(mine >= 0), starts = __ballot(mine >= 0 && (lane == 0 || prev < 0 || prev + 1 != mine || mine % 16 == 0));
+    const int side = 64 / cpr, my = lane / cpr, c = lane - my * cpr, n_starts = __popcll(starts);   // groups side by side (cpr <= 32)
+    for (int at = 0; at < n_starts; at += side) {
+        uint64_t left = starts;
+        for (int k = 0; k < at + my; ++k) left &= left - 1;           // (my group: the at + my'th)
+        const bool mine_too = my < side && left != 0;
+        const int i = mine_too ? __builtin_ctzll(left) : 0;
+        const int64_t s0 = __shfl(mine, i, 64);
+        if (!mine_too) continue;
+        uint64_t stop = i < 63 ? ((starts | ~there) >> (i + 1)) : 0;
+        const int n = min(stop ? __builtin_ctzll(stop) + 1 : 64 - i, win - i);
+        const int64_t page = s0 >> v.ps;
         const int first = (int)(s0 & 15);
-        for (int d = lane; d < dim; d += 64) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(codes + (int64_t)d * P);
+        const float sc = a.vscale[page * a.Hkv + h];
+        const uint8_t* codes = (const uint8_t*)a.vcodes + (page * a.Hkv + h) * (int64_t)P * dim + (int64_t)(8 * c) * P + (s0 & (P - 1) & ~15);
+        u32x4 w[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float x[4];
-                from_codes<CODE>(w[e], x);
+        for (int e = 0; e < 8; ++e) w[e] = *reinterpret_cast<const u32x4*>(codes + e * P);
+        E* dst = (E*)a.v + (w0 + i - first) * a.ldv + (int64_t)h * a.v_head_stride + 8 * c;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int k = 4 * e + j - first;
-                    if (k >= 0 && k < n) dst[k * a.ldv + d] = from_f32<E>(x[j] * sc);
-                }
+        for (int q = 0; q < 4; ++q) {
+            float x[8][4];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) from_codes<CODE>(w[e][q], x[e]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = 4 * q + j;
+                if (k < first || k >= first + n) continue;
+                float o[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = x[e][j] * sc;
+                put8(dst + k * a.ldv, o);
             }
         }
     }
@@ -454,11 +514,18 @@ PCB_EXPORT int pcb_page_tables(const pcb_page_tables_args* a, void* stream) {
             hipLaunchKernelGGL((KERNEL<float, PCB_CODE_INT8>), GRID, dim3(256), 0, (hipStream_t)stream, *a, __VA_ARGS__);        \
     } while (0)
 
+// rows that a wave looks at: as many as leave the chip's 1024 SIMDs two waves each or more, at most 64
+static int window(int n_rows, int Hkv, int least, int most) {
+    int w = least;
+    while (w < most && (int64_t)n_rows * Hkv * 2 / (2 * w) >= 4096) w *= 2;
+    return w;
+}
+
 PCB_EXPORT int pcb_pages_append(const pcb_pages_rows_args* a, void* stream) {
     const int rc = check_rows(a, "pcb_pages_append");
     if (rc != PCB_OK || a->n_rows == 0) return rc;
     const RowsView v{a->row_slot, a->n_rows, pcb_log2(a->page_size), (int64_t)a->n_pages * a->page_size};
-    const int win = (int64_t)a->n_rows * a->Hkv <= 16384 ? 1 : 16;      // rows of different requests side by side; or prompts, whose windows start at most a page or two
+    const int win = window(a->n_rows, a->Hkv, 1, a->page_size < 64 ? 32 : 64);   // (rows of different requests side by side; prompts: a page or two start in a window)
     const int64_t waves = ((int64_t)a->n_rows + win - 1) / win * a->Hkv;
     const dim3 grid((unsigned)((waves + 3) / 4), 2);
     PCB_PAGES_LAUNCH(pages_append_kernel, grid, v, win);
@@ -469,8 +536,9 @@ PCB_EXPORT int pcb_pages_read(const pcb_pages_rows_args* a, void* stream) {
     const int rc = check_rows(a, "pcb_pages_read");
     if (rc != PCB_OK || a->n_rows == 0) return rc;
     const RowsView v{a->row_slot, a->n_rows, pcb_log2(a->page_size), (int64_t)a->n_pages * a->page_size};
-    const int64_t waves = ((int64_t)a->n_rows + 15) / 16 * a->Hkv;
+    const int win = window(a->n_rows, a->Hkv, 4, 32);
+    const int64_t waves = ((int64_t)a->n_rows + win - 1) / win * a->Hkv;
     const dim3 grid((unsigned)((waves + 3) / 4), 2);
-    PCB_PAGES_LAUNCH(pages_read_kernel, grid, v);
+    PCB_PAGES_LAUNCH(pages_read_kernel, grid, v, win);
     return pcb_check_launch("pages_read_kernel");
 }
