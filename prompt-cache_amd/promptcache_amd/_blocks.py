@@ -1184,15 +1184,21 @@ def rec_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lds_, reqs: torc
 
 
 # ---- keys and values in 8 bits, in pages ------------------------------------------------------------------------------------------------------
+# (A step calls these once a layer, and a short step's kernel is over before the next call is made: good arguments are recognised in as few looks as there are tensors, and
+# only what is not taken is looked at again for what to say.)
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+_raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 def _flat(t: Optional[torch.Tensor], dtype, numel: int, dev: int, what: str) -> Optional[int]:
     """The address of ``t`` (optional), which holds at least ``numel`` elements of ``dtype`` one after the other on device ``dev``."""
     if t is None:
         return None
-    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous() or t.numel() < numel:
-        if t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
-            _want(t, dtype, what)
-        raise ValueError(f"{what}: {numel} elements on cuda:{dev} are needed, got {t.numel()} on {t.device}")
-    return t.data_ptr()
+    if t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and t.numel() >= numel:
+        return t.data_ptr()
+    if t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
+        _want(t, dtype, what)
+    raise ValueError(f"{what}: {numel} elements on cuda:{dev} are needed, got {t.numel()} on {t.device}")
 
 
 def _device_of(t: torch.Tensor, what: str) -> int:
@@ -1200,22 +1206,28 @@ def _device_of(t: torch.Tensor, what: str) -> int:
     dev = t.get_device()
     if dev < 0:
         raise TypeError(f"{what}: need a device tensor, got one on {t.device}")
-    if dev != torch.cuda.current_device():
-        raise ValueError(f"{what} lies on {t.device}, and the current device is cuda:{torch.cuda.current_device()}")
+    if dev != _device():
+        raise ValueError(f"{what} lies on {t.device}, and the current device is cuda:{_device()}")
     return dev
 
 
 def _pool(kcodes: torch.Tensor, kscale: torch.Tensor, vcodes: torch.Tensor, vscale: torch.Tensor, dev: int, what: str):
-    """Checks a pool: codes ``[pages, Hkv, P, dim]`` / ``[pages, Hkv, dim, P]``, scales ``[pages, Hkv]``; -> (code, its pointers, (pages, P), (Hkv, dim))."""
-    code = CODES.get(kcodes.dtype)
-    if code is None or vcodes.dtype is not kcodes.dtype:
-        raise TypeError(f"{what}: codes are both float8_e4m3fn or both int8, got {kcodes.dtype} and {vcodes.dtype}")
-    if kcodes.dim() != 4 or vcodes.shape != (kcodes.shape[0], kcodes.shape[1], kcodes.shape[3], kcodes.shape[2]):
-        raise ValueError(f"{what}: key codes [pages, heads, P, dim] and value codes [pages, heads, dim, P], got {tuple(kcodes.shape)} and {tuple(vcodes.shape)}")
-    pages, Hkv, P, dim = kcodes.shape
-    ptrs = (_flat(kcodes, kcodes.dtype, 0, dev, "key codes of " + what), _flat(kscale, torch.float32, pages * Hkv, dev, "key scales of " + what),
-            _flat(vcodes, kcodes.dtype, 0, dev, "value codes of " + what), _flat(vscale, torch.float32, pages * Hkv, dev, "value scales of " + what))
-    return code, ptrs, (pages, P), (Hkv, dim)
+    """Checks a pool: codes ``[pages, Hkv, P, dim]`` / ``[pages, Hkv, dim, P]``, scales ``[pages, Hkv]``; -> (code, pages, P, Hkv, dim)."""
+    dtype = kcodes.dtype
+    code = CODES.get(dtype)
+    if code is None or vcodes.dtype is not dtype:
+        raise TypeError(f"{what}: codes are both float8_e4m3fn or both int8, got {dtype} and {vcodes.dtype}")
+    shape = kcodes.shape
+    if len(shape) != 4 or vcodes.shape != (shape[0], shape[1], shape[3], shape[2]):
+        raise ValueError(f"{what}: key codes [pages, heads, P, dim] and value codes [pages, heads, dim, P], got {tuple(shape)} and {tuple(vcodes.shape)}")
+    pages, Hkv, P, dim = shape
+    if not (kcodes.is_contiguous() and vcodes.is_contiguous() and kcodes.get_device() == dev and vcodes.get_device() == dev):
+        _flat(kcodes, dtype, 0, dev, "key codes of " + what), _flat(vcodes, dtype, 0, dev, "value codes of " + what)
+    n = pages * Hkv
+    if not (kscale.dtype is _F32 and vscale.dtype is _F32 and kscale.is_contiguous() and vscale.is_contiguous() and kscale.numel() >= n and vscale.numel() >= n
+            and kscale.get_device() == dev and vscale.get_device() == dev):
+        _flat(kscale, _F32, n, dev, "key scales of " + what), _flat(vscale, _F32, n, dev, "value scales of " + what)
+    return code, pages, P, Hkv, dim
 
 
 def _heads(t: torch.Tensor, heads: int, dim: int, dev: int, what: str):
@@ -1228,9 +1240,13 @@ def _heads(t: torch.Tensor, heads: int, dim: int, dev: int, what: str):
 
 def _table(table: torch.Tensor, n: int, dev: int, what: str):
     """An int32 block table of at least ``n`` contiguous rows; -> (address, row stride, pages)."""
-    if table.dim() != 2 or table.shape[0] < n or table.dtype is not torch.int32 or table.stride(1) != 1 and table.numel() > 0 or table.get_device() != dev:
-        raise ValueError(f"{what}: a table int32 [{n}, pages] on cuda:{dev} with contiguous rows, got {table.dtype} {tuple(table.shape)} on {table.device}")
-    return table.data_ptr(), max(table.stride(0), table.shape[1]) if table.shape[0] < 2 else table.stride(0), table.shape[1]
+    shape, stride = table.shape, table.stride()
+    if len(shape) != 2 or shape[0] < n or table.dtype is not _I32 or stride[1] != 1 and table.numel() > 0 or table.get_device() != dev:
+        raise ValueError(f"{what}: a table int32 [{n}, pages] on cuda:{dev} with contiguous rows, got {table.dtype} {tuple(shape)} on {table.device}")
+    return table.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], shape[1]), shape[1]
+
+
+_TABLES_BYTES, _ROWS_BYTES, _ATTN_BYTES = C.sizeof(PageTablesArgs), C.sizeof(PagesRowsArgs), C.sizeof(AttnPagesArgs)
 
 
 def page_tables(cached: torch.Tensor, brings: torch.Tensor, table: torch.Tensor, page_size: int, *, row_slot: torch.Tensor, kv_len=None, row_start=None, row_seq=None,
@@ -1239,27 +1255,34 @@ def page_tables(cached: torch.Tensor, brings: torch.Tensor, table: torch.Tensor,
     and brings (below zero: it is over); ``table`` int32 [n, max_pages] gets the pages taken from ``ring`` (int32, the free pages; ``ring_state`` int32 [2 or
     more] {first, number}; ``ring_out`` int32 [4], may be ``ring_state``).  ``row_slot`` int64 [rows] and, optional, ``row_seq`` / ``row_pos`` int32 [rows],
     ``row_start`` [n + 1], ``kv_len`` [n], ``tiles`` [n + rows // tile_rows, 4], ``status`` [2] are written; without ``ring`` the table holds all pages already."""
-    n, rows, i32 = cached.numel(), row_slot.numel(), torch.int32
+    n, rows = cached.numel(), row_slot.numel()
     dev = _device_of(cached, "page_tables cached")
     tab, ld, pages = _table(table, n, dev, "page_tables")
-    a = PageTablesArgs(C.sizeof(PageTablesArgs), n, pages, ld, page_size, _flat(cached, i32, n, dev, "cached"), _flat(brings, i32, n, dev, "brings"),
-                       _flat(keep, i32, n, dev, "keep"), tab, _flat(ring, i32, 1, dev, "ring"), 0 if ring is None else ring.numel(),
-                       _flat(ring_state, i32, 2, dev, "ring_state"), _flat(ring_out, i32, 4, dev, "ring_out"), _flat(kv_len, i32, n, dev, "kv_len"),
-                       _flat(row_start, i32, n + 1, dev, "row_start"), _flat(row_seq, i32, rows, dev, "row_seq"), _flat(row_pos, i32, rows, dev, "row_pos"),
-                       _flat(row_slot, torch.int64, rows, dev, "row_slot"), rows, _flat(tiles, i32, 0, dev, "tiles"), 0 if tiles is None else tiles.numel() // 4, tile_rows,
-                       _flat(status, i32, 2, dev, "status"))
-    check(load().pcb_page_tables(C.byref(a), _stream()), "pcb_page_tables")
+    a = PageTablesArgs(_TABLES_BYTES, n, pages, ld, page_size, _flat(cached, _I32, n, dev, "cached"), _flat(brings, _I32, n, dev, "brings"), _flat(keep, _I32, n, dev, "keep"),
+                       tab, _flat(ring, _I32, 1, dev, "ring"), 0 if ring is None else ring.numel(), _flat(ring_state, _I32, 2, dev, "ring_state"),
+                       _flat(ring_out, _I32, 4, dev, "ring_out"), _flat(kv_len, _I32, n, dev, "kv_len"), _flat(row_start, _I32, n + 1, dev, "row_start"),
+                       _flat(row_seq, _I32, rows, dev, "row_seq"), _flat(row_pos, _I32, rows, dev, "row_pos"), _flat(row_slot, _I64, rows, dev, "row_slot"), rows,
+                       _flat(tiles, _I32, 0, dev, "tiles"), 0 if tiles is None else tiles.numel() // 4, tile_rows, _flat(status, _I32, 2, dev, "status"))
+    rc = (_lib or load()).pcb_page_tables(a, _raw_stream(dev))
+    if rc:
+        check(rc, "pcb_page_tables")
 
 
 def _pages_rows(name: str, k, v, row_slot, kcodes, kscale, vcodes, vscale) -> None:
-    code, ptrs, (pages, P), (Hkv, dim) = _pool(kcodes, kscale, vcodes, vscale, k.get_device(), name)
-    dev = _device_of(k, name)
-    if k.dtype is not v.dtype or k.shape != v.shape:
+    dev = k.get_device()
+    code, pages, P, Hkv, dim = _pool(kcodes, kscale, vcodes, vscale, dev, name)
+    if dev < 0 or dev != _device():
+        _device_of(k, name)
+    shape = k.shape
+    if k.dtype is not v.dtype or shape != v.shape:
         raise TypeError(f"{name}: keys and values of one type and shape, got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
-    rows = k.shape[0]
-    a = PagesRowsArgs(C.sizeof(PagesRowsArgs), _code(k), code, *_heads(k, Hkv, dim, dev, name), *_heads(v, Hkv, dim, dev, name),
-                      _flat(row_slot, torch.int64, rows, dev, "row_slot of " + name), rows, *ptrs, pages, P, Hkv, dim)
-    check(getattr(load(), "pcb_" + name)(C.byref(a), _stream()), name)
+    rows = shape[0]
+    a = PagesRowsArgs(_ROWS_BYTES, _code(k), code, *_heads(k, Hkv, dim, dev, name), *_heads(v, Hkv, dim, dev, name), _flat(row_slot, _I64, rows, dev, "row_slot"), rows,
+                      kcodes.data_ptr(), kscale.data_ptr(), vcodes.data_ptr(), vscale.data_ptr(), pages, P, Hkv, dim)
+    lib = _lib or load()
+    rc = (lib.pcb_pages_append if name == "pages_append" else lib.pcb_pages_read)(a, _raw_stream(dev))
+    if rc:
+        check(rc, name)
 
 
 def pages_append(k: torch.Tensor, v: torch.Tensor, row_slot: torch.Tensor, kcodes: torch.Tensor, kscale: torch.Tensor, vcodes: torch.Tensor, vscale: torch.Tensor) -> None:
@@ -1286,19 +1309,24 @@ def attn_pages(q: torch.Tensor, tiles: torch.Tensor, tile_rows: int, kv_len: tor
     """Causal attention of rows ``q`` [rows, H, dim] over the pages of ``table`` int32 [n, max_pages], ``kv_len`` int32 [n] tokens of which are written; ``tiles`` int32
     [t, 4] {sequence, first position, rows, first flat row} as ``page_tables`` makes them, of at most ``tile_rows`` rows; ``sink`` fp32 [H].  ``longest``: an upper bound
     of ``kv_len`` known to the host (0: the table's width); ``part`` fp32 of ``attn_pages_part(...)`` floats (None: allocated when it is needed)."""
-    code, ptrs, (pages, P), (Hkv, dim) = _pool(kcodes, kscale, vcodes, vscale, q.get_device(), "attn_pages")
-    dev = _device_of(q, "attn_pages queries")
-    if q.dim() != 3 or out.shape != q.shape or out.dtype is not q.dtype or q.shape[1] % Hkv:
-        raise ValueError(f"attn_pages: queries and results [rows, H, {dim}], H a multiple of {Hkv}, of one type; got {q.dtype} {tuple(q.shape)} and {out.dtype} {tuple(out.shape)}")
-    rows, H = q.shape[0], q.shape[1]
+    dev = q.get_device()
+    code, pages, P, Hkv, dim = _pool(kcodes, kscale, vcodes, vscale, dev, "attn_pages")
+    if dev < 0 or dev != _device():
+        _device_of(q, "attn_pages queries")
+    shape = q.shape
+    if len(shape) != 3 or out.shape != shape or out.dtype is not q.dtype or shape[1] % Hkv:
+        raise ValueError(f"attn_pages: queries and results [rows, H, {dim}], H a multiple of {Hkv}, of one type; got {q.dtype} {tuple(shape)} and {out.dtype} {tuple(out.shape)}")
+    rows, H, _ = shape
     n, n_tiles = kv_len.numel(), tiles.numel() // 4
     tab, ld, wide = _table(table, n, dev, "attn_pages")
     longest = longest if longest > 0 else wide * P
     if part is None:
         floats = attn_pages_part(rows, H, Hkv, dim, n_tiles, tile_rows, longest)
-        part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    a = AttnPagesArgs(C.sizeof(AttnPagesArgs), _code(q), code, *_heads(q, H, dim, dev, "attn_pages queries"), _flat(tiles, torch.int32, 0, dev, "attn_pages tiles"), n_tiles,
-                      tile_rows, rows, _flat(kv_len, torch.int32, 0, dev, "attn_pages kv_len"), tab, ld, n, wide, *ptrs, pages, P, H, Hkv, dim, float(scale), int(window),
-                      _flat(sink, torch.float32, H, dev, "attn_pages sink"), *_heads(out, H, dim, dev, "attn_pages results"), longest,
-                      _flat(part, torch.float32, 0, dev, "attn_pages part"), 0 if part is None else part.numel())
-    check(load().pcb_attn_pages(C.byref(a), _stream()), "pcb_attn_pages")
+        part = torch.empty(floats, dtype=_F32, device=q.device) if floats else None
+    a = AttnPagesArgs(_ATTN_BYTES, _code(q), code, *_heads(q, H, dim, dev, "attn_pages queries"), _flat(tiles, _I32, 0, dev, "attn_pages tiles"), n_tiles, tile_rows, rows,
+                      _flat(kv_len, _I32, 0, dev, "attn_pages kv_len"), tab, ld, n, wide, kcodes.data_ptr(), kscale.data_ptr(), vcodes.data_ptr(), vscale.data_ptr(), pages, P, H,
+                      Hkv, dim, scale, window, _flat(sink, _F32, H, dev, "attn_pages sink"), *_heads(out, H, dim, dev, "attn_pages results"), longest,
+                      _flat(part, _F32, 0, dev, "attn_pages part"), 0 if part is None else part.numel())
+    rc = (_lib or load()).pcb_attn_pages(a, _raw_stream(dev))
+    if rc:
+        check(rc, "pcb_attn_pages")
