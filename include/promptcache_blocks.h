@@ -943,7 +943,9 @@ int pcb_pages_read(const pcb_pages_rows_args* a, void* stream);
  *   out = sum_j e^(scale q.k_j) v_j / (sum_j e^(scale q.k_j) + e^sink[h]),   sink (fp32 [H]) optional; a row that sees nothing: 0
  * Query head h reads key head h / (H / Hkv).  scale > 0.  Tiles without rows or of no sequence, and rows outside [0, n_rows), are passed over.
  * longest: an upper bound of kv_len that the host knows (0: max_pages * P, which pcb_attn_pages_part is then given); it decides the number of key runs that workgroups of their own take, whose
- * results need part: pcb_attn_pages_part(...) floats, aligned to 16 bytes; launches that may run at the same time need a part of their own. */
+ * results need part: pcb_attn_pages_part(...) floats, aligned to 16 bytes.  counters (int32 [512], optional): zero before the first launch that is given them and left zero
+ * by every launch; with them a tile of few columns is merged by the last of its workgroups, without them (and tiles of many) in a second launch.  Launches that may run at
+ * the same time need a part and counters of their own. */
 typedef struct pcb_attn_pages_args {
     uint32_t struct_bytes;
     int32_t dtype, code;
@@ -969,6 +971,7 @@ typedef struct pcb_attn_pages_args {
     int32_t longest;
     float* part;
     int64_t part_floats;
+    int32_t* counters;
 } pcb_attn_pages_args;
 int64_t pcb_attn_pages_part(int32_t n_rows, int32_t H, int32_t Hkv, int32_t dim, int32_t n_tiles, int32_t tile_rows, int32_t longest);
 int pcb_attn_pages(const pcb_attn_pages_args* a, void* stream);

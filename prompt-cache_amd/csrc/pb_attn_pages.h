@@ -10,7 +10,7 @@ constexpr float NEG = -__builtin_inff();
 
 constexpr int MANY_COLS = 128;
 constexpr int MAX_GROUPS = 512;        // workgroups that share out the steps: two a CU
-constexpr int SHARED_TILES = 1024;     // tiles whose work is shared out evenly; more are enough units by themselves
+constexpr int SHARED_TILES = 512;      // tiles whose work is shared out evenly; more are enough units by themselves
 constexpr int UNIT_STEPS = 6;          // what a unit costs beside its steps (queries, the first loads, the end), in steps
 
 struct Plan {

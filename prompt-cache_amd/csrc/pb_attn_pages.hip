@@ -26,41 +26,36 @@ __device__ __forceinline__ float sum4(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 
-// The lane's part of a query row as operands, sixteen neighbouring elements for each 64: two k-steps of 32.  -> the power of two that the row was divided by.
+// The lane's part of a query row: sixteen neighbouring elements for each 64, as they are in memory
+template <typename E, int DB>
+struct Query {
+    u32x4 w[DB][sizeof(E)];
+};
+template <typename E, int DB>
+__device__ __forceinline__ void load_query(Query<E, DB>& q, const E* p, int dim, int g) {
+#pragma unroll
+    for (int c = 0; c < DB; ++c)
+#pragma unroll
+        for (int k = 0; k < (int)sizeof(E); ++k) q.w[c][k] = *reinterpret_cast<const u32x4*>(p + min(64 * c + 16 * g, dim - 16) + k * (16 / sizeof(E)));
+}
+// .. as operands, two k-steps of 32 for each 64 elements, zeros behind the row's end and where the column is nobody's.  -> the power of two that the row was divided by: its largest
+// element becomes 2^14 .. 2^15, and what is 2^-28 of that is still a normal half
 template <typename E, int DB, int PARTS>
-__device__ __forceinline__ float load_query(const E* p, int dim, int g, bool live, h8 (&qf)[PARTS][2 * DB]) {
-    float x[DB][16], m = 0.0f;
+__device__ __forceinline__ float operands(const Query<E, DB>& q, int dim, int g, bool live, h8 (&qf)[PARTS][2 * DB]) {
+    auto at = [&](int c, int e) {
+        float x;
+        if constexpr (sizeof(E) == 2)
+            x = __uint_as_float(e & 1 ? q.w[c][e >> 3][(e & 7) >> 1] & 0xffff0000u : q.w[c][e >> 3][(e & 7) >> 1] << 16);
+        else
+            x = __uint_as_float(q.w[c][e >> 2][e & 3]);
+        return live && 64 * c + 16 * g < dim ? x : 0.0f;
+    };
+    float m = 0.0f;
 #pragma unroll
     for (int c = 0; c < DB; ++c)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[c][e] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < DB; ++c) {
-        const int d = 64 * c + 16 * g;
-        if (live && d < dim) {
-            if constexpr (sizeof(E) == 2) {
-                const u32x4 a = *reinterpret_cast<const u32x4*>(p + d), b = *reinterpret_cast<const u32x4*>(p + d + 8);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[c][2 * e] = __uint_as_float(a[e] << 16), x[c][2 * e + 1] = __uint_as_float(a[e] & 0xffff0000u);
-                    x[c][8 + 2 * e] = __uint_as_float(b[e] << 16), x[c][9 + 2 * e] = __uint_as_float(b[e] & 0xffff0000u);
-                }
-            } else {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const f4 a = *reinterpret_cast<const f4*>(p + d + 4 * q);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[c][4 * q + e] = a[e];
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int c = 0; c < DB; ++c)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) m = fmaxf(m, __builtin_fabsf(x[c][e]) < __builtin_inff() ? __builtin_fabsf(x[c][e]) : 0.0f);
+        for (int e = 0; e < 16; ++e) m = fmaxf(m, __builtin_fabsf(at(c, e)) < __builtin_inff() ? __builtin_fabsf(at(c, e)) : 0.0f);
     m = max4(m);
-    // the row's largest element becomes 2^14 .. 2^15: what is 2^-28 of it is still a normal half
     int e2 = (int)(__float_as_uint(m) >> 23) - 127 - 14;
     e2 = e2 < -110 ? -110 : e2;
     const float inv = __uint_as_float((uint32_t)(127 - e2) << 23), unit = __uint_as_float((uint32_t)(127 + e2) << 23);
@@ -68,7 +63,7 @@ __device__ __forceinline__ float load_query(const E* p, int dim, int g, bool liv
     for (int c = 0; c < DB; ++c)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const float y = x[c][e] * inv;
+            const float y = at(c, e) * inv;
             const _Float16 hi = (_Float16)y;
             qf[0][2 * c + (e >> 3)][e & 7] = hi;
             if constexpr (PARTS == 2) qf[1][2 * c + (e >> 3)][e & 7] = __builtin_fabsf(y) < __builtin_inff() ? (_Float16)(y - (float)hi) : (_Float16)0.0f;
@@ -114,6 +109,15 @@ __device__ __forceinline__ void weights(f4 (&acc)[4], float f, float vs, float& 
     l = l * alpha + sum;
 }
 
+// Numbers that one workgroup leaves for another one of the same launch: written through and read past the caches, which differ between XCDs.
+__device__ __forceinline__ void hand_on(float* p, float x, float y) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), (uint64_t)__float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 handed(const float* p) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return float2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
+}
+
 // A unit is 16 NC columns of a tile and one key head.  The steps of all units, one after the other, are shared out evenly: a workgroup's share may begin inside a unit and
 // end inside another one; what is not a whole unit goes to `part`.  So sequences of any lengths fill the chip alike, and no workgroup starts in vain.  A unit without steps
 // counts as one: its rows get their zeros.
@@ -127,7 +131,8 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
     constexpr int NW = 4, NT = 256, PARTS = F32 ? 2 : 1, NB = 4 * DB, COLS = 16 * NC;   // NB: value column blocks of 16
     __shared__ __attribute__((aligned(16))) float Os[NW][16][64 * DB + 4];
     __shared__ float Ms[NW][COLS], Ls[NW][COLS];
-    __shared__ int starts[SHARED_TILES + 1], wsum[NW];
+    __shared__ __attribute__((aligned(16))) int4 tiles_s[SHARED_TILES];
+    __shared__ int starts[SHARED_TILES + 1], kv_s[SHARED_TILES], wsum[NW], last_s;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int per = pl.per, dim = a.dim, ps = pl.ps, P = 1 << ps;
     const int64_t plane = (int64_t)P * dim;
@@ -141,6 +146,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
             int n = 0;
             if (t0 + tid < a.n_tiles) {
                 const Tile x = tile_of(a, t0 + tid, ps);
+                tiles_s[t0 + tid] = int4{x.seq, x.pos, x.rows, x.row0}, kv_s[t0 + tid] = x.kv;
                 n = (max(x.s1 - x.s0, 1) + UNIT_STEPS) * a.Hkv * ((x.rows * per + COLS - 1) / COLS);
             }
             int v = n;
@@ -166,7 +172,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
         share = share < NW + UNIT_STEPS ? NW + UNIT_STEPS : share;
         if (tid == 0) starts[a.n_tiles] = all;
         __syncthreads();
-        if (blockIdx.x == 0) {                                        // for the launch that merges
+        if (blockIdx.x == 0 && !a.counters) {                         // for the launch that merges
             int* head = reinterpret_cast<int*>(a.part);
             for (int t = tid; t <= a.n_tiles; t += NT) head[t] = starts[t];
             if (tid == 0) head[a.n_tiles + 1] = share;
@@ -176,7 +182,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
     const int at0 = at;
     float* const part = a.part + head_floats(a.n_tiles);
     while (at < end) {
-        int t, j, from, steps, n_steps, mine = 1;                     // unit j of tile t, its steps from .. from + n_steps - 1
+        int t, j, from, steps, n_steps, mine = 1, g0 = 0, parts = 1, second = 0;  // unit j of tile t, its steps from .. from + n_steps - 1; the workgroups that share it are g0 ..
         Tile tl;
         if (pl.groups) {
             int lo = 0, hi = a.n_tiles;
@@ -188,12 +194,16 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
                     hi = mid;
             }
             t = __builtin_amdgcn_readfirstlane(lo);
-            tl = tile_of(a, t, ps);
+            const int4 rec = tiles_s[t];
+            tl.seq = __builtin_amdgcn_readfirstlane(rec.x), tl.pos = __builtin_amdgcn_readfirstlane(rec.y), tl.rows = __builtin_amdgcn_readfirstlane(rec.z);
+            tl.row0 = __builtin_amdgcn_readfirstlane(rec.w), tl.kv = __builtin_amdgcn_readfirstlane(kv_s[t]);
+            tl = rows_of(a, tl, 0, tl.rows - 1);
             steps = max(tl.s1 - tl.s0, 1);
             const int off = at - __builtin_amdgcn_readfirstlane(starts[t]), cost = steps + UNIT_STEPS;
             j = off / cost;
             const int p = off - j * cost;
             mine = min(cost - p, end - at);
+            g0 = (at - p + UNIT_STEPS) / share, parts = (at - p + cost - 1) / share - g0 + 1, second = at - p > g0 * share;
             from = max(p - UNIT_STEPS, 0), n_steps = max(p + mine - UNIT_STEPS, 0) - from;
         } else {
             t = blockIdx.x, j = blockIdx.y;
@@ -247,6 +257,13 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
 #pragma unroll
             for (int b = 0; b < NB; ++b) vr[b] = *reinterpret_cast<const u32x4*>(p + 16 * min(b, last_b) * P);
         };
+        // (the queries are asked for first: loads arrive in order, and they are made operands while the first keys are under way)
+        Query<E, DB> raw[NC];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const int col = min(col0 + 16 * n + c, rows * per - 1), qr = row_of(pl, col), h = hk * per + col - qr * per;
+            load_query<E, DB>(raw[n], (const E*)a.q + ((int64_t)tl.row0 + qr) * a.ldq + (int64_t)h * a.q_head_stride, dim, g);
+        }
         int s = s0 + wave, i = 0;
         if (s < s1) {
             look(s);
@@ -256,9 +273,9 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
         for (int n = 0; n < NC; ++n) {
             const int col = col0 + 16 * n + c;
             const bool live = col < rows * per;
-            const int qr = live ? row_of(pl, col) : 0, h = hk * per + (live ? col - qr * per : 0), pos = live ? tl.pos + qr : -1;
+            const int pos = live ? tl.pos + row_of(pl, col) : -1;
             lo[n] = a.window > 0 ? pos - a.window + 1 : 0, hi[n] = min(kv, pos + 1);
-            const float unit2 = load_query<E, DB, PARTS>((const E*)a.q + ((int64_t)tl.row0 + qr) * a.ldq + (int64_t)h * a.q_head_stride, dim, g, live, qf[n]);
+            const float unit2 = operands<E, DB, PARTS>(raw[n], dim, g, live, qf[n]);
             qs[n] = F32 ? unit2 * a.scale : unit2 * (a.scale * LOG2E);  // bf16: scores in units of ln 2
         }
         float M[NC], l[NC];
@@ -372,7 +389,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
             float* pp = part + (int64_t)slot * COLS * (dim + 2);
             E* op = (E*)a.out + ((int64_t)tl.row0 + qr) * a.ldo + (int64_t)h * a.out_head_stride;
             const float f = unit ? finished<E>(a, h, m, den, 16384.0f) * (1.0f / 16384.0f) : 1.0f;
-            if (!unit && (tid & 15) == 0) *reinterpret_cast<float2*>(pp + COLS * dim + 2 * (16 * n + cc)) = float2{m, den};
+            if (!unit && (tid & 15) == 0) hand_on(pp + COLS * dim + 2 * (16 * n + cc), m, den);
             for (int d = 4 * (tid & 15); d < dim; d += 64) {
                 f4 v = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -380,8 +397,74 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
                 if (unit)
                     store4(op + d, v[0] * f, v[1] * f, v[2] * f, v[3] * f);
                 else
-                    *reinterpret_cast<f4*>(pp + (16 * n + cc) * dim + d) = v;
+                    hand_on(pp + (16 * n + cc) * dim + d, v[0], v[1]), hand_on(pp + (16 * n + cc) * dim + d + 2, v[2], v[3]);
             }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // (every wave's results have left it before one of them answers for all)
+        __syncthreads();
+        if (unit || !a.counters) continue;
+        // The last of the unit's workgroups merges: its fellows' results were past the caches before they were counted.
+        if (tid == 0) {
+            last_s = __hip_atomic_fetch_add(&a.counters[g0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+            if (last_s) __hip_atomic_store(&a.counters[g0], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!last_s) continue;
+        // Sixteen threads a column, and more sets of sixteen where there are fewer columns: each adds up every so many of the results under a running maximum, then the sets' sums are
+        // put together.  (A wave a column instead, its maximum first: 32 columns of 15 results 18 us longer than the second launch that this saves.)
+        const int64_t result = (int64_t)COLS * (dim + 2);
+        auto place = [&](int i) { return part + (2 * (int64_t)(g0 + i) + (i == 0 ? second : 0)) * result; };
+        auto add = [&](float& m, float& den, f4 (&v)[DB], float mi, float li, const f4 (&vi)[DB]) {
+            const float mn = fmaxf(m, mi), mu = mn == NEG ? 0.0f : mn, x = pow_of<E>(m - mu), y = pow_of<E>(mi - mu);
+            m = mn, den = den * x + li * y;
+#pragma unroll
+            for (int k = 0; k < DB; ++k) v[k] = v[k] * x + vi[k] * y;
+        };
+        float* sums = &Os[0][0][0];                                   // [16][64 DB + 4]
+        for (int n = 0; n < NC; ++n) {
+            const int n_live = min(16, rows * per - col0 - 16 * n);
+            if (n_live <= 0) break;
+            const int wide = n_live == 1 ? 1 : 1 << (32 - __builtin_clz(n_live - 1)), grp = tid >> 4, q = tid & 15;   // (a power of two of columns)
+            const int cc = 16 * n + (grp & (wide - 1)), set = grp / wide, sets = 16 / wide;
+            float m = NEG, den = 0.0f;
+            f4 v[DB];
+#pragma unroll
+            for (int k = 0; k < DB; ++k) v[k] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (int i = set; i < parts; i += sets) {
+                const float* p = place(i);
+                const float2 x = handed(p + COLS * dim + 2 * cc);
+                f4 w[DB];
+#pragma unroll
+                for (int k = 0; k < DB; ++k) {
+                    const int d = min(4 * q + 64 * k, dim - 4);
+                    const float2 y = handed(p + cc * dim + d), z = handed(p + cc * dim + d + 2);
+                    w[k] = f4{y.x, y.y, z.x, z.y};
+                }
+                add(m, den, v, x.x, x.y, w);
+            }
+            float* mine_s = sums + grp * (64 * DB + 4);
+            if (sets > 1) {
+                __syncthreads();                                      // (`sums` of the columns before have been read)
+#pragma unroll
+                for (int k = 0; k < DB; ++k) *reinterpret_cast<f4*>(mine_s + 4 * q + 64 * k) = v[k];
+                if (q == 0) mine_s[64 * DB] = m, mine_s[64 * DB + 1] = den;
+                __syncthreads();
+                for (int k = 1; k < sets && set == 0; ++k) {
+                    const float* o = sums + (grp + k * wide) * (64 * DB + 4);
+                    f4 w[DB];
+#pragma unroll
+                    for (int e = 0; e < DB; ++e) w[e] = *reinterpret_cast<const f4*>(o + 4 * q + 64 * e);
+                    add(m, den, v, o[64 * DB], o[64 * DB + 1], w);
+                }
+            }
+            if (set > 0 || cc - 16 * n >= n_live) continue;
+            const int col = col0 + cc, qr = row_of(pl, col), h = hk * per + col - qr * per;
+            const float f = finished<E>(a, h, m, den, 16384.0f) * (1.0f / 16384.0f);
+            E* op = (E*)a.out + ((int64_t)tl.row0 + qr) * a.ldo + (int64_t)h * a.out_head_stride;
+#pragma unroll
+            for (int k = 0; k < DB; ++k)
+                if (4 * q + 64 * k < dim) store4(op + 4 * q + 64 * k, v[k][0] * f, v[k][1] * f, v[k][2] * f, v[k][3] * f);
         }
         __syncthreads();
     }
@@ -471,6 +554,12 @@ Plan plan_of(int64_t H, int Hkv, int dim, int n_tiles, int tile_rows, int64_t lo
     }
     return p;
 }
+// Whether a unit's results are merged by the last of its workgroups: while these are few, a second launch costs more (us, two launches / one; 1 to 512 units of 4 columns and 1 to 64
+// results 17.6 / 15.0 to 194 / 190, 16 columns of 5 results 18.1 / 15.8, but of 32 16.9 / 18.3)
+bool merged_in_launch(const Plan& p, int Hkv, int n_tiles, int tile_rows) {
+    const int64_t cols = (int64_t)tile_rows * p.per, units = (int64_t)n_tiles * Hkv * p.cblocks;
+    return (cols < p.cols ? cols : p.cols) * (p.groups / units + 1) < 256;
+}
 int64_t part_floats(const Plan& p, int Hkv, int dim, int n_tiles) {
     if (p.cols == MANY_COLS) return p.runs > 1 ? (int64_t)n_tiles * Hkv * p.cblocks * p.runs * MANY_COLS * (dim + 2) : 0;
     return p.groups ? head_floats(n_tiles) + 2 * (int64_t)p.groups * p.cols * (dim + 2) : 0;
@@ -498,7 +587,7 @@ int dispatch(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
         launch_rows<E, CODE, 2>(a, pl, stream);
     else
         launch_rows<E, CODE, 4>(a, pl, stream);
-    if (pl.groups || pl.runs > 1) hipLaunchKernelGGL(attn_pages_merge_kernel<E>, dim3(a.n_tiles, a.H, a.tile_rows < 32 ? a.tile_rows : 32), dim3(256), 0, stream, a, pl);
+    if ((pl.groups && !a.counters) || pl.runs > 1) hipLaunchKernelGGL(attn_pages_merge_kernel<E>, dim3(a.n_tiles, a.H, a.tile_rows < 32 ? a.tile_rows : 32), dim3(256), 0, stream, a, pl);
     return pcb_check_launch("attn_pages_rows_kernel");
 }
 
@@ -534,7 +623,10 @@ PCB_EXPORT int pcb_attn_pages(const pcb_attn_pages_args* a, void* stream) {
                 "pcb_attn_pages: too many tiles, heads or tile rows (heads times tile rows up to 2^20, 2048 query heads a key head)");
     PCB_REQUIRE((!p.groups && p.runs == 1) || (a->part && (uintptr_t)a->part % 16 == 0 && a->part_floats >= part_floats(p, a->Hkv, a->dim, a->n_tiles)), PCB_ERR_ARG,
                 "pcb_attn_pages: shared key runs need pcb_attn_pages_part floats");
+    PCB_REQUIRE((uintptr_t)a->counters % 4 == 0, PCB_ERR_ARG, "pcb_attn_pages: counters are whole numbers");
+    pcb_attn_pages_args b = *a;
+    if (!merged_in_launch(p, a->Hkv, a->n_tiles, a->tile_rows)) b.counters = nullptr;
     if (a->dtype == PCB_BF16)
-        return a->code == PCB_CODE_E4M3 ? dispatch<bf16_t, PCB_CODE_E4M3>(*a, p, (hipStream_t)stream) : dispatch<bf16_t, PCB_CODE_INT8>(*a, p, (hipStream_t)stream);
-    return a->code == PCB_CODE_E4M3 ? dispatch<float, PCB_CODE_E4M3>(*a, p, (hipStream_t)stream) : dispatch<float, PCB_CODE_INT8>(*a, p, (hipStream_t)stream);
+        return a->code == PCB_CODE_E4M3 ? dispatch<bf16_t, PCB_CODE_E4M3>(b, p, (hipStream_t)stream) : dispatch<bf16_t, PCB_CODE_INT8>(b, p, (hipStream_t)stream);
+    return a->code == PCB_CODE_E4M3 ? dispatch<float, PCB_CODE_E4M3>(b, p, (hipStream_t)stream) : dispatch<float, PCB_CODE_INT8>(b, p, (hipStream_t)stream);
 }

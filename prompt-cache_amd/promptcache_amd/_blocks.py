@@ -233,7 +233,7 @@ class AttnPagesArgs(C.Structure):
                 ("kv_len", _vp), ("table", _vp), ("ld_table", _i64), ("n_seqs", _i32), ("max_pages", _i32),
                 ("kcodes", _vp), ("kscale", _vp), ("vcodes", _vp), ("vscale", _vp), ("n_pages", _i32), ("page_size", _i32),
                 ("H", _i32), ("Hkv", _i32), ("dim", _i32), ("scale", _f32), ("window", _i32), ("sink", _vp),
-                ("out", _vp), ("ldo", _i64), ("out_head_stride", _i64), ("longest", _i32), ("part", _vp), ("part_floats", _i64)]
+                ("out", _vp), ("ldo", _i64), ("out_head_stride", _i64), ("longest", _i32), ("part", _vp), ("part_floats", _i64), ("counters", _vp)]
 
 
 # name -> (restype, argtypes); mirrors include/promptcache_blocks.h one to one
@@ -1304,11 +1304,25 @@ def attn_pages_part(rows: int, H: int, Hkv: int, dim: int, n_tiles: int, tile_ro
     return int(n)
 
 
+_counters = {}
+
+
+def _stream_counters(dev: int, stream: int, device) -> Optional[torch.Tensor]:
+    """Counters for launches that follow one another on a stream: zero between them.  None while the stream is captured."""
+    if torch.cuda.is_current_stream_capturing():
+        return None
+    t = _counters.get((dev, stream))
+    if t is None:
+        t = _counters[dev, stream] = torch.zeros(512, dtype=_I32, device=device)
+    return t
+
+
 def attn_pages(q: torch.Tensor, tiles: torch.Tensor, tile_rows: int, kv_len: torch.Tensor, table: torch.Tensor, kcodes: torch.Tensor, kscale: torch.Tensor,
-               vcodes: torch.Tensor, vscale: torch.Tensor, out: torch.Tensor, *, scale: float, window: int = 0, sink=None, longest: int = 0, part=None) -> None:
+               vcodes: torch.Tensor, vscale: torch.Tensor, out: torch.Tensor, *, scale: float, window: int = 0, sink=None, longest: int = 0, part=None, counters=None) -> None:
     """Causal attention of rows ``q`` [rows, H, dim] over the pages of ``table`` int32 [n, max_pages], ``kv_len`` int32 [n] tokens of which are written; ``tiles`` int32
     [t, 4] {sequence, first position, rows, first flat row} as ``page_tables`` makes them, of at most ``tile_rows`` rows; ``sink`` fp32 [H].  ``longest``: an upper bound
-    of ``kv_len`` known to the host (0: the table's width); ``part`` fp32 of ``attn_pages_part(...)`` floats (None: allocated when it is needed)."""
+    of ``kv_len`` known to the host (0: the table's width); ``part`` fp32 of ``attn_pages_part(...)`` floats (None: allocated when it is needed); ``counters`` int32 [512], zero
+    before their first call and for calls that follow one another (None: those that this module keeps for the stream, or none in a capture, whose replays may run beside others)."""
     dev = q.get_device()
     code, pages, P, Hkv, dim = _pool(kcodes, kscale, vcodes, vscale, dev, "attn_pages")
     if dev < 0 or dev != _device():
@@ -1323,10 +1337,13 @@ def attn_pages(q: torch.Tensor, tiles: torch.Tensor, tile_rows: int, kv_len: tor
     if part is None:
         floats = attn_pages_part(rows, H, Hkv, dim, n_tiles, tile_rows, longest)
         part = torch.empty(floats, dtype=_F32, device=q.device) if floats else None
+    stream = _raw_stream(dev)
+    if counters is None and part is not None:
+        counters = _stream_counters(dev, stream, q.device)
     a = AttnPagesArgs(_ATTN_BYTES, _code(q), code, *_heads(q, H, dim, dev, "attn_pages queries"), _flat(tiles, _I32, 0, dev, "attn_pages tiles"), n_tiles, tile_rows, rows,
                       _flat(kv_len, _I32, 0, dev, "attn_pages kv_len"), tab, ld, n, wide, kcodes.data_ptr(), kscale.data_ptr(), vcodes.data_ptr(), vscale.data_ptr(), pages, P, H,
                       Hkv, dim, scale, window, _flat(sink, _F32, H, dev, "attn_pages sink"), *_heads(out, H, dim, dev, "attn_pages results"), longest,
-                      _flat(part, _F32, 0, dev, "attn_pages part"), 0 if part is None else part.numel())
-    rc = (_lib or load()).pcb_attn_pages(a, _raw_stream(dev))
+                      _flat(part, _F32, 0, dev, "attn_pages part"), 0 if part is None else part.numel(), _flat(counters, _I32, 512, dev, "attn_pages counters"))
+    rc = (_lib or load()).pcb_attn_pages(a, stream)
     if rc:
         check(rc, "pcb_attn_pages")

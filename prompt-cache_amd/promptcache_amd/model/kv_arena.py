@@ -455,6 +455,7 @@ class PageCache:
         self.ring = torch.arange(pages, dtype=torch.int32, device=device)
         self.ring_state = torch.tensor([0, pages, 0, 0], dtype=torch.int32, device=device)
         self._bufs, self._outgrown, self._shared = {}, [], False
+        self._counters = torch.zeros(512, dtype=torch.int32, device=device)   # (steps of one cache follow one another)
 
     def bytes_per_token(self) -> float:
         """Bytes that one token takes, its part of the scales with it."""
@@ -513,7 +514,7 @@ class PageCache:
         floats = B.attn_pages_part(step.rows, q.shape[1], g, d, step.tiles.shape[0], step.tile_rows, longest)
         part = self._buf("part", (floats,), torch.float32) if floats else None
         B.attn_pages(q, step.tiles, step.tile_rows, step.kv_len, self.table, self.kcodes[layer], self.kscale[layer], self.vcodes[layer], self.vscale[layer], out,
-                     scale=d ** -0.5 if scale is None else scale, window=window, sink=sink, longest=longest, part=part)
+                     scale=d ** -0.5 if scale is None else scale, window=window, sink=sink, longest=longest, part=part, counters=self._counters)
         return out
 
     def share(self, source: int, target: int, tokens: int) -> None:
