@@ -244,11 +244,10 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && DB <= 2 ? 2 : 1) void attn_p
             }
             M = M_new;
 #pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const _Float16* v = &Vs[buf][(32 * d + c) * VLD + 8 * hh];
+            for (int m = 0; m < 4; ++m) {
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    const h8 x = *reinterpret_cast<const h8*>(v + 16 * m);
+                for (int d = 0; d < ND; ++d) {
+                    const h8 x = *reinterpret_cast<const h8*>(&Vs[buf][(32 * d + c) * VLD + 8 * hh + 16 * m]);
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wf[p][m], o[d], 0, 0, 0);
                 }
