@@ -118,6 +118,15 @@ __device__ __forceinline__ float2 handed(const float* p) {
     return float2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
 }
 
+// one more result of a column: maximum, denominator, sums
+template <typename E, int DB>
+__device__ __forceinline__ void add_result(float& m, float& den, f4 (&v)[DB], float mi, float li, const f4 (&vi)[DB]) {
+    const float mn = fmaxf(m, mi), mu = mn == NEG ? 0.0f : mn, x = pow_of<E>(m - mu), y = pow_of<E>(mi - mu);
+    m = mn, den = den * x + li * y;
+#pragma unroll
+    for (int k = 0; k < DB; ++k) v[k] = v[k] * x + vi[k] * y;
+}
+
 // A unit is 16 NC columns of a tile and one key head.  The steps of all units, one after the other, are shared out evenly: a workgroup's share may begin inside a unit and
 // end inside another one; what is not a whole unit goes to `part`.  So sequences of any lengths fill the chip alike, and no workgroup starts in vain.  A unit without steps
 // counts as one: its rows get their zeros.
@@ -414,12 +423,6 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
         // put together.  (A wave a column instead, its maximum first: 32 columns of 15 results 18 us longer than the second launch that this saves.)
         const int64_t result = (int64_t)COLS * (dim + 2);
         auto place = [&](int i) { return part + (2 * (int64_t)(g0 + i) + (i == 0 ? second : 0)) * result; };
-        auto add = [&](float& m, float& den, f4 (&v)[DB], float mi, float li, const f4 (&vi)[DB]) {
-            const float mn = fmaxf(m, mi), mu = mn == NEG ? 0.0f : mn, x = pow_of<E>(m - mu), y = pow_of<E>(mi - mu);
-            m = mn, den = den * x + li * y;
-#pragma unroll
-            for (int k = 0; k < DB; ++k) v[k] = v[k] * x + vi[k] * y;
-        };
         float* sums = &Os[0][0][0];                                   // [16][64 DB + 4]
         for (int n = 0; n < NC; ++n) {
             const int n_live = min(16, rows * per - col0 - 16 * n);
@@ -441,7 +444,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
                     const float2 y = handed(p + cc * dim + d), z = handed(p + cc * dim + d + 2);
                     w[k] = f4{y.x, y.y, z.x, z.y};
                 }
-                add(m, den, v, x.x, x.y, w);
+                add_result<E, DB>(m, den, v, x.x, x.y, w);
             }
             float* mine_s = sums + grp * (64 * DB + 4);
             if (sets > 1) {
@@ -455,7 +458,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
                     f4 w[DB];
 #pragma unroll
                     for (int e = 0; e < DB; ++e) w[e] = *reinterpret_cast<const f4*>(o + 4 * q + 64 * e);
-                    add(m, den, v, o[64 * DB], o[64 * DB + 1], w);
+                    add_result<E, DB>(m, den, v, o[64 * DB], o[64 * DB + 1], w);
                 }
             }
             if (set > 0 || cc - 16 * n >= n_live) continue;
@@ -470,67 +473,68 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
     }
 }
 
-// One workgroup a (tile, head, row): the results of the workgroups that shared the row's unit under one maximum.  Their factors once (a lane each), then groups of dim / 4 threads
-// add up every so many of them.
-template <typename E>
-__global__ __launch_bounds__(256) void attn_pages_merge_kernel(pcb_attn_pages_args a, Plan pl) {
-    __shared__ float fac[MAX_GROUPS];
-    __shared__ f4 sums[256];
-    __shared__ float inv_s;
-    const int h = blockIdx.y, dim = a.dim, tid = threadIdx.x, lane = tid & 63, t = blockIdx.x;
+// The results of the workgroups that shared a unit, put together in a launch of their own: sixteen threads a (row, head), or `sets` times as many where there are many results, each
+// adds up every so many of them under a running maximum.
+template <typename E, int DB>
+__global__ __launch_bounds__(256) void attn_pages_merge_kernel(pcb_attn_pages_args a, Plan pl, int sets) {
+    __shared__ __attribute__((aligned(16))) float sums[16][64 * DB + 4];
+    const int dim = a.dim, per = pl.per, grp = threadIdx.x >> 4, q = threadIdx.x & 15, wide = 16 / sets, set = grp / wide;
+    const int blocks = (a.tile_rows * a.H + wide - 1) / wide, t = blockIdx.x / blocks, item = (blockIdx.x - t * blocks) * wide + (grp & (wide - 1)), r = item / a.H, h = item - r * a.H;
     const Tile tl = tile_of(a, t, pl.ps);
-    const int per = pl.per, quads = dim / 4, groups = 256 / quads, grp = tid / quads, quad = tid % quads;
     const bool many = pl.cols == MANY_COLS;
     const int* head = reinterpret_cast<const int*>(a.part);
-    const int start = many ? 0 : head[t], share = many ? 1 : head[a.n_tiles + 1];
     const float* part = many ? a.part : a.part + head_floats(a.n_tiles);
     const int64_t result = (int64_t)pl.cols * (dim + 2);
-    for (int r = blockIdx.z; r < tl.rows; r += gridDim.z) {
-        const int col = r * per + h % per, cc = col % pl.cols, cblock = col / pl.cols, hk = h / per;
-        int64_t first;                                                // the place of the unit's first result, and that of its second
-        int64_t second;
-        int n;
+    const int hk = row_of(pl, h), col = r * per + h - hk * per, cblock = col / pl.cols, cc = col - cblock * pl.cols;
+    int64_t first, second, apart;                                     // the places of the unit's first result, of its second, and from there to the next
+    int n = 0;
+    if (r < tl.rows) {
         if (many) {
             const Tile bl = rows_of(a, tl, row_of(pl, cblock * MANY_COLS), row_of(pl, min(cblock * MANY_COLS + MANY_COLS, tl.rows * per) - 1));
             n = min((bl.s1 - bl.s0 + pl.run - 1) / pl.run, pl.runs);
-            first = (((int64_t)t * a.Hkv + hk) * pl.cblocks + cblock) * pl.runs, second = first + 1;
+            first = (((int64_t)t * a.Hkv + hk) * pl.cblocks + cblock) * pl.runs, second = first + 1, apart = 1;
         } else {
-            const int steps = max(tl.s1 - tl.s0, 1), u0 = start + (steps + UNIT_STEPS) * (cblock * a.Hkv + hk), s0 = u0 + UNIT_STEPS;   // the unit's and its first step's place among all
+            const int share = head[a.n_tiles + 1];
+            const int steps = max(tl.s1 - tl.s0, 1), u0 = head[t] + (steps + UNIT_STEPS) * (cblock * a.Hkv + hk), s0 = u0 + UNIT_STEPS;   // the unit's and its first step's place among all
             const int g0 = s0 / share;
             n = (s0 + steps - 1) / share - g0 + 1;
-            first = 2 * (int64_t)g0 + (u0 > g0 * share ? 1 : 0), second = 2 * ((int64_t)g0 + 1);
-        }
-        if (n <= 1) continue;                                         // (one workgroup had it all)
-        const int64_t apart = many ? 1 : 2;
-        auto place = [&](int i) { return part + (i == 0 ? first : second + apart * (i - 1)) * result; };
-        __syncthreads();
-        if (tid < 64) {
-            float m = NEG, den = 0.0f;
-            for (int i = lane; i < n; i += 64) m = fmaxf(m, place(i)[pl.cols * dim + 2 * cc]);
-            m = wave_max(m);
-            const float mu = m == NEG ? 0.0f : m;
-            for (int i = lane; i < n; i += 64) {
-                const float2 x = *reinterpret_cast<const float2*>(place(i) + pl.cols * dim + 2 * cc);
-                const float f = pow_of<E>(x.x - mu);
-                fac[i] = f;
-                den += x.y * f;
-            }
-            den = wave_sum(den);
-            if (lane == 0) inv_s = finished<E>(a, h, m, den, 16384.0f);
-        }
-        __syncthreads();
-        f4 v = f4{0.f, 0.f, 0.f, 0.f};
-        if (grp < groups)
-#pragma unroll 4
-            for (int i = grp; i < n; i += groups) v += *reinterpret_cast<const f4*>(place(i) + cc * dim + 4 * quad) * fac[i];
-        sums[tid] = v;
-        __syncthreads();
-        if (tid < quads) {
-            for (int k = 1; k < groups; ++k) v += sums[k * quads + quad];
-            v *= inv_s * (1.0f / 16384.0f);
-            store4((E*)a.out + ((int64_t)tl.row0 + r) * a.ldo + (int64_t)h * a.out_head_stride + 4 * quad, v[0], v[1], v[2], v[3]);
+            first = 2 * (int64_t)g0 + (u0 > g0 * share ? 1 : 0), second = 2 * ((int64_t)g0 + 1), apart = 2;
         }
     }
+    n = n <= 1 ? 0 : n;                                               // (one workgroup had it all)
+    float m = NEG, den = 0.0f;
+    f4 v[DB];
+#pragma unroll
+    for (int k = 0; k < DB; ++k) v[k] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = set; i < n; i += sets) {
+        const float* p = part + (i == 0 ? first : second + apart * (i - 1)) * result;
+        const float2 x = *reinterpret_cast<const float2*>(p + pl.cols * dim + 2 * cc);
+        f4 w[DB];
+#pragma unroll
+        for (int k = 0; k < DB; ++k) w[k] = *reinterpret_cast<const f4*>(p + cc * dim + min(4 * q + 64 * k, dim - 4));
+        add_result<E, DB>(m, den, v, x.x, x.y, w);
+    }
+    if (sets > 1) {
+        float* mine = sums[grp];
+#pragma unroll
+        for (int k = 0; k < DB; ++k) *reinterpret_cast<f4*>(mine + 4 * q + 64 * k) = v[k];
+        if (q == 0) mine[64 * DB] = m, mine[64 * DB + 1] = den;
+        __syncthreads();
+        for (int k = 1; k < sets && set == 0; ++k) {
+            const float* o = sums[grp + k * wide];
+            f4 w[DB];
+#pragma unroll
+            for (int e = 0; e < DB; ++e) w[e] = *reinterpret_cast<const f4*>(o + 4 * q + 64 * e);
+            add_result<E, DB>(m, den, v, o[64 * DB], o[64 * DB + 1], w);
+        }
+    }
+    if (n == 0 || set > 0) return;
+    const float f = finished<E>(a, h, m, den, 16384.0f) * (1.0f / 16384.0f);
+    E* op = (E*)a.out + ((int64_t)tl.row0 + r) * a.ldo + (int64_t)h * a.out_head_stride;
+#pragma unroll
+    for (int k = 0; k < DB; ++k)
+        if (4 * q + 64 * k < dim) store4(op + 4 * q + 64 * k, v[k][0] * f, v[k][1] * f, v[k][2] * f, v[k][3] * f);
 }
 
 // How a call is cut.  Up to 32 columns a tile: in blocks of 16 or 32, the steps of everything shared out; more: blocks of 128, in key runs where these are too few to fill
@@ -576,6 +580,13 @@ void launch_rows(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t strea
     hipLaunchKernelGGL((attn_pages_rows_kernel<E, CODE, DB, 1>), grid, block, 0, stream, a, pl);
 }
 
+template <typename E, int DB>
+void launch_merge(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
+    const int64_t units = (int64_t)a.n_tiles * a.Hkv * pl.cblocks, results = pl.cols == MANY_COLS ? pl.runs : pl.groups / units + 1;
+    const int sets = results > 32 ? 16 : results > 16 ? 8 : results > 8 ? 4 : results > 4 ? 2 : 1, wide = 16 / sets;
+    hipLaunchKernelGGL((attn_pages_merge_kernel<E, DB>), dim3((unsigned)(a.n_tiles * (((int64_t)a.tile_rows * a.H + wide - 1) / wide))), dim3(256), 0, stream, a, pl, sets);
+}
+
 template <typename E, int CODE>
 int dispatch(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
     if (pl.cols == MANY_COLS) {
@@ -585,9 +596,18 @@ int dispatch(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
         launch_rows<E, CODE, 1>(a, pl, stream);
     else if (a.dim <= 128)
         launch_rows<E, CODE, 2>(a, pl, stream);
+    else if (a.dim <= 192)
+        launch_rows<E, CODE, 3>(a, pl, stream);
     else
         launch_rows<E, CODE, 4>(a, pl, stream);
-    if ((pl.groups && !a.counters) || pl.runs > 1) hipLaunchKernelGGL(attn_pages_merge_kernel<E>, dim3(a.n_tiles, a.H, a.tile_rows < 32 ? a.tile_rows : 32), dim3(256), 0, stream, a, pl);
+    if ((pl.groups && !a.counters) || pl.runs > 1) {
+        if (a.dim <= 64)
+            launch_merge<E, 1>(a, pl, stream);
+        else if (a.dim <= 128)
+            launch_merge<E, 2>(a, pl, stream);
+        else
+            launch_merge<E, 4>(a, pl, stream);
+    }
     return pcb_check_launch("attn_pages_rows_kernel");
 }
 
@@ -616,11 +636,15 @@ PCB_EXPORT int pcb_attn_pages(const pcb_attn_pages_args* a, void* stream) {
                 PCB_ERR_ARG, "pcb_attn_pages: rows, heads, codes and tiles start on 16 bytes");
     const int64_t longest = a->longest > 0 ? a->longest : (int64_t)a->max_pages * a->page_size;
     Plan p = plan_of(a->H, a->Hkv, a->dim, a->n_tiles, a->tile_rows, longest);
+    if (a->window > 0 && (int64_t)a->window + a->tile_rows + 62 < longest) {   // no tile sees more keys than this: fewer runs, never more scratch
+        const Plan w = plan_of(a->H, a->Hkv, a->dim, a->n_tiles, a->tile_rows, (int64_t)a->window + a->tile_rows + 62);
+        if (part_floats(w, a->Hkv, a->dim, a->n_tiles) <= part_floats(p, a->Hkv, a->dim, a->n_tiles)) p = w;
+    }
     p.ps = pcb_log2(a->page_size);
     // (costs are counted in 31 bits; whoever has more of them has enough units)
     if (p.groups && (int64_t)a->n_tiles * a->Hkv * p.cblocks > 0x7fffffff / ((int64_t)a->max_pages * a->page_size / 64 + 2 + UNIT_STEPS) - MAX_GROUPS) p.groups = 0;
-    PCB_REQUIRE((int64_t)a->Hkv * p.cblocks <= 65535 && p.per <= 2048 && a->H <= 65535 && a->n_tiles < 1 << 23 && (p.cols != MANY_COLS || (int64_t)a->n_tiles * a->Hkv * p.cblocks < 1 << 23), PCB_ERR_ARG,
-                "pcb_attn_pages: too many tiles, heads or tile rows (heads times tile rows up to 2^20, 2048 query heads a key head)");
+    PCB_REQUIRE((int64_t)a->Hkv * p.cblocks <= 65535 && p.per <= 2048 && (int64_t)a->tile_rows * a->H <= 1 << 19 && a->H <= 65535 && a->n_tiles < 1 << 23 && (p.cols != MANY_COLS || (int64_t)a->n_tiles * a->Hkv * p.cblocks < 1 << 23), PCB_ERR_ARG,
+                "pcb_attn_pages: too many tiles, heads or tile rows (heads times tile rows up to 2^19, 2048 query heads a key head)");
     PCB_REQUIRE((!p.groups && p.runs == 1) || (a->part && (uintptr_t)a->part % 16 == 0 && a->part_floats >= part_floats(p, a->Hkv, a->dim, a->n_tiles)), PCB_ERR_ARG,
                 "pcb_attn_pages: shared key runs need pcb_attn_pages_part floats");
     PCB_REQUIRE((uintptr_t)a->counters % 4 == 0, PCB_ERR_ARG, "pcb_attn_pages: counters are whole numbers");

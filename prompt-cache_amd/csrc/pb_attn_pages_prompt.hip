@@ -5,7 +5,7 @@
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_f16: a lane owns one column, its 32 scores of a step are its own operand of the second product (row 8 i + 4 h + j of the
 // first product's operand is key 16 (i / 2) + 8 h + 4 (i % 2) + j of 32, so lane half h holds keys 16 m + 8 h .. + 7), and a column's maximum is one exchange between two lanes.
 //
-// LDS rows are 16 bytes longer than their 64 DB halves of a key, or 64 keys of a value column: the sixteen lanes that are served at once fall on all banks.
+// LDS rows are 16 bytes longer than their 32 ND halves of a key, or 64 keys of a value column: the sixteen lanes that are served at once fall on all banks.
 #include "pb_attn_pages.h"
 
 namespace {
@@ -24,12 +24,13 @@ __device__ __forceinline__ float sum2(float v) {
 }
 __device__ __forceinline__ float lane_of(float v, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)); }
 
-template <typename E, int CODE, int DB>
-__global__ __launch_bounds__(256, sizeof(E) == 2 && DB <= 2 ? 2 : 1) void attn_pages_prompt_kernel(pcb_attn_pages_args a, Plan pl) {
+// ND: value columns (and key elements) in blocks of 32
+template <typename E, int CODE, int ND>
+__global__ __launch_bounds__(256, sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_pages_prompt_kernel(pcb_attn_pages_args a, Plan pl) {
     constexpr bool F32 = sizeof(E) == 4;
-    constexpr int PARTS = F32 ? 2 : 1, KK = 4 * DB, ND = 2 * DB;      // k-steps of 16 of the first product, row blocks of 32 of the second
-    constexpr int KLD = 64 * DB + 8, VLD = 72;
-    __shared__ __attribute__((aligned(16))) _Float16 Ks[2][64 * KLD], Vs[2][64 * DB * VLD];
+    constexpr int PARTS = F32 ? 2 : 1, KK = 2 * ND;                   // k-steps of 16 of the first product
+    constexpr int KLD = 32 * ND + 8, VLD = 72, PIECES = 128 * ND, NP = (PIECES + 255) / 256;   // sixteen-byte pieces of a step's keys, and of its values; of each a thread's
+    __shared__ __attribute__((aligned(16))) _Float16 Ks[2][64 * KLD], Vs[2][32 * ND * VLD];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, c = lane & 31;
     const int hk = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, cb = rest % pl.cblocks, t = a.n_tiles - 1 - rest / pl.cblocks;   // (a prompt's last tiles, which see most keys, first)
     const int dim = a.dim, ps = pl.ps, P = 1 << ps, per = pl.per;
@@ -59,13 +60,13 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && DB <= 2 ? 2 : 1) void attn_p
         const int64_t ph = (int64_t)(pages < 0 ? 0 : pages) * a.Hkv + hk;
         kss = pages < 0 ? 1.0f : a.kscale[ph], vss = pages < 0 ? 1.0f : a.vscale[ph];
     };
-    // staging: thread t takes 16-byte pieces t, t + 256, .. of the step's keys (4 DB a row) and of its value columns (four a column, the same sixteen keys each time)
+    // staging: thread t takes pieces t, t + 256, .. of the step's keys (2 ND a row) and of its value columns (four a column, the same sixteen keys each time)
     const int vq = tid & 3;
-    u32x4 kr[DB], vr[DB];
+    u32x4 kr[NP], vr[NP];
     auto fetch = [&](int s, int i) {
 #pragma unroll
-        for (int n = 0; n < DB; ++n) {
-            const int row = (n * 256 + tid) / (4 * DB), ch = tid % (4 * DB);
+        for (int n = 0; n < NP; ++n) {
+            const int piece = min(n * 256 + tid, PIECES - 1), row = piece / (2 * ND), ch = piece % (2 * ND);
             const int page = __shfl(pages, 4 * i + (row >> 4), 64);
             const uint8_t* p = (const uint8_t*)a.kcodes + ((int64_t)(page < 0 ? 0 : page) * a.Hkv + hk) * plane + ((s * 64 + row) & (P - 1)) * dim;
             kr[n] = *reinterpret_cast<const u32x4*>(p + 16 * min(ch, dim / 16 - 1));
@@ -73,7 +74,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && DB <= 2 ? 2 : 1) void attn_p
         const int page = __shfl(pages, 4 * i + vq, 64);
         const uint8_t* p = (const uint8_t*)a.vcodes + ((int64_t)(page < 0 ? 0 : page) * a.Hkv + hk) * plane + ((s * 64 + 16 * vq) & (P - 1));
 #pragma unroll
-        for (int n = 0; n < DB; ++n) vr[n] = *reinterpret_cast<const u32x4*>(p + min(n * 64 + (tid >> 2), dim - 1) * P);
+        for (int n = 0; n < NP; ++n) vr[n] = *reinterpret_cast<const u32x4*>(p + min(n * 64 + (tid >> 2), dim - 1) * P);
         // values behind the last written key are whatever the memory held, and no number times 0 is 0 for all of them
         const int have = page < 0 ? 0 : kv - (s * 64 + 16 * vq);
         if (have < 16) {
@@ -82,14 +83,15 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && DB <= 2 ? 2 : 1) void attn_p
                 const int k = have - 4 * e;
                 const uint32_t keep = k >= 4 ? 0xffffffffu : k <= 0 ? 0u : 0xffffffffu >> (32 - 8 * k);
 #pragma unroll
-                for (int n = 0; n < DB; ++n) vr[n][e] &= keep;
+                for (int n = 0; n < NP; ++n) vr[n][e] &= keep;
             }
         }
     };
     auto stage = [&](int buf) {
 #pragma unroll
-        for (int n = 0; n < DB; ++n) {
-            const int row = (n * 256 + tid) / (4 * DB), ch = tid % (4 * DB);
+        for (int n = 0; n < NP; ++n) {
+            if (PIECES % 256 && n * 256 + tid >= PIECES) break;
+            const int row = (n * 256 + tid) / (2 * ND), ch = (n * 256 + tid) % (2 * ND);
             _Float16* k = &Ks[buf][row * KLD + 16 * ch];
             *reinterpret_cast<h8*>(k) = half8<CODE>(u32x2{kr[n][0], kr[n][1]});
             *reinterpret_cast<h8*>(k + 8) = half8<CODE>(u32x2{kr[n][2], kr[n][3]});
@@ -279,12 +281,17 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && DB <= 2 ? 2 : 1) void attn_p
 template <typename E, int CODE>
 int launch(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
     const dim3 grid((unsigned)((int64_t)a.n_tiles * a.Hkv * pl.cblocks), pl.runs), block(256);
-    if (a.dim <= 64)
-        hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 1>), grid, block, 0, stream, a, pl);
-    else if (a.dim <= 128)
+    const int blocks = (a.dim + 31) / 32;
+    if (blocks <= 2)
         hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 2>), grid, block, 0, stream, a, pl);
-    else
+    else if (blocks == 3)
+        hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 3>), grid, block, 0, stream, a, pl);
+    else if (blocks == 4)
         hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 4>), grid, block, 0, stream, a, pl);
+    else if (blocks <= 6)
+        hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 6>), grid, block, 0, stream, a, pl);
+    else
+        hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 8>), grid, block, 0, stream, a, pl);
     return pcb_check_launch("attn_pages_prompt_kernel");
 }
 
