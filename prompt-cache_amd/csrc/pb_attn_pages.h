@@ -21,7 +21,7 @@ struct Plan {
     int runs, run;                     // many columns (cols = 128): key runs of a unit and their steps
 };
 // what `part` holds.  Few columns: the sums of the tiles' costs (int32 [n_tiles + 1]) and a workgroup's share, then for two results of each workgroup [cols][dim] and [cols][2];
-// many columns: the same of each run of each unit
+// many columns: [dim] of each run of each (flat row, head), then all their pairs
 __host__ __device__ inline int64_t head_floats(int n_tiles) { return ((int64_t)n_tiles + 2 + 3) / 4 * 4; }
 
 // x / per for x per < 2^32

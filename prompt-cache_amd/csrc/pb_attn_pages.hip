@@ -481,25 +481,27 @@ __global__ __launch_bounds__(256) void attn_pages_merge_kernel(pcb_attn_pages_ar
     const int dim = a.dim, per = pl.per, grp = threadIdx.x >> 4, q = threadIdx.x & 15, wide = 16 / sets, set = grp / wide;
     const int blocks = (a.tile_rows * a.H + wide - 1) / wide, t = blockIdx.x / blocks, item = (blockIdx.x - t * blocks) * wide + (grp & (wide - 1)), r = item / a.H, h = item - r * a.H;
     const Tile tl = tile_of(a, t, pl.ps);
-    const bool many = pl.cols == MANY_COLS;
-    const int* head = reinterpret_cast<const int*>(a.part);
-    const float* part = many ? a.part : a.part + head_floats(a.n_tiles);
-    const int64_t result = (int64_t)pl.cols * (dim + 2);
     const int hk = row_of(pl, h), col = r * per + h - hk * per, cblock = col / pl.cols, cc = col - cblock * pl.cols;
-    int64_t first, second, apart;                                     // the places of the unit's first result, of its second, and from there to the next
+    // the column's first result (sums, maximum and denominator), its second, and how far it is from there to the next
+    const float *sum0 = a.part, *sum1 = a.part, *max0 = a.part, *max1 = a.part;
+    int64_t sum_step = 0, max_step = 0;
     int n = 0;
-    if (r < tl.rows) {
-        if (many) {
-            const Tile bl = rows_of(a, tl, row_of(pl, cblock * MANY_COLS), row_of(pl, min(cblock * MANY_COLS + MANY_COLS, tl.rows * per) - 1));
-            n = min((bl.s1 - bl.s0 + pl.run - 1) / pl.run, pl.runs);
-            first = (((int64_t)t * a.Hkv + hk) * pl.cblocks + cblock) * pl.runs, second = first + 1, apart = 1;
-        } else {
-            const int share = head[a.n_tiles + 1];
-            const int steps = max(tl.s1 - tl.s0, 1), u0 = head[t] + (steps + UNIT_STEPS) * (cblock * a.Hkv + hk), s0 = u0 + UNIT_STEPS;   // the unit's and its first step's place among all
-            const int g0 = s0 / share;
-            n = (s0 + steps - 1) / share - g0 + 1;
-            first = 2 * (int64_t)g0 + (u0 > g0 * share ? 1 : 0), second = 2 * ((int64_t)g0 + 1), apart = 2;
-        }
+    if (r < tl.rows && pl.cols == MANY_COLS) {
+        const Tile bl = rows_of(a, tl, row_of(pl, cblock * MANY_COLS), row_of(pl, min(cblock * MANY_COLS + MANY_COLS, tl.rows * per) - 1));
+        n = min((bl.s1 - bl.s0 + pl.run - 1) / pl.run, pl.runs);
+        const int64_t i = (((int64_t)tl.row0 + r) * a.H + h) * pl.runs;
+        sum0 = a.part + i * dim, max0 = a.part + (int64_t)a.n_rows * a.H * pl.runs * dim + 2 * i;
+        sum1 = sum0 + dim, max1 = max0 + 2, sum_step = dim, max_step = 2;
+    } else if (r < tl.rows) {
+        const int* head = reinterpret_cast<const int*>(a.part);
+        const float* part = a.part + head_floats(a.n_tiles);
+        const int64_t result = (int64_t)pl.cols * (dim + 2);
+        const int share = head[a.n_tiles + 1];
+        const int steps = max(tl.s1 - tl.s0, 1), u0 = head[t] + (steps + UNIT_STEPS) * (cblock * a.Hkv + hk), s0 = u0 + UNIT_STEPS;   // the unit's and its first step's place among all
+        const int g0 = s0 / share;
+        n = (s0 + steps - 1) / share - g0 + 1;
+        const float *first = part + (2 * (int64_t)g0 + (u0 > g0 * share ? 1 : 0)) * result, *second = part + 2 * ((int64_t)g0 + 1) * result;
+        sum0 = first + cc * dim, max0 = first + pl.cols * dim + 2 * cc, sum1 = second + cc * dim, max1 = second + pl.cols * dim + 2 * cc, sum_step = max_step = 2 * result;
     }
     n = n <= 1 ? 0 : n;                                               // (one workgroup had it all)
     float m = NEG, den = 0.0f;
@@ -508,11 +510,11 @@ __global__ __launch_bounds__(256) void attn_pages_merge_kernel(pcb_attn_pages_ar
     for (int k = 0; k < DB; ++k) v[k] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int i = set; i < n; i += sets) {
-        const float* p = part + (i == 0 ? first : second + apart * (i - 1)) * result;
-        const float2 x = *reinterpret_cast<const float2*>(p + pl.cols * dim + 2 * cc);
+        const float *p = i == 0 ? sum0 : sum1 + sum_step * (i - 1), *mp = i == 0 ? max0 : max1 + max_step * (i - 1);
+        const float2 x = *reinterpret_cast<const float2*>(mp);
         f4 w[DB];
 #pragma unroll
-        for (int k = 0; k < DB; ++k) w[k] = *reinterpret_cast<const f4*>(p + cc * dim + min(4 * q + 64 * k, dim - 4));
+        for (int k = 0; k < DB; ++k) w[k] = *reinterpret_cast<const f4*>(p + min(4 * q + 64 * k, dim - 4));
         add_result<E, DB>(m, den, v, x.x, x.y, w);
     }
     if (sets > 1) {
@@ -539,18 +541,22 @@ __global__ __launch_bounds__(256) void attn_pages_merge_kernel(pcb_attn_pages_ar
 
 // How a call is cut.  Up to 32 columns a tile: in blocks of 16 or 32, the steps of everything shared out; more: blocks of 128, in key runs where these are too few to fill
 // the chip.
-Plan plan_of(int64_t H, int Hkv, int dim, int n_tiles, int tile_rows, int64_t longest) {
+Plan plan_of(int64_t n_rows, int64_t H, int Hkv, int dim, int n_tiles, int tile_rows, int64_t longest) {
     Plan p{};
     p.per = (int)(H / Hkv);
     p.magic = p.per > 1 ? (uint32_t)(((1ull << 32) + p.per - 1) / p.per) : 0;
     const int64_t cols = (int64_t)tile_rows * p.per, steps = (longest + 63) / 64 > 0 ? (longest + 63) / 64 : 1;
     p.cols = tile_rows > 1 && cols > 32 ? MANY_COLS : cols <= 16 || dim > 128 ? 16 : 32;
     p.cblocks = (int)(cols > 1 << 30 ? 1 << 26 : (cols + p.cols - 1) / p.cols);
-    const int64_t units = (int64_t)n_tiles * Hkv * p.cblocks;
+    int64_t units = (int64_t)n_tiles * Hkv * p.cblocks;
     p.runs = 1, p.run = 1 << 30;
     if (p.cols == MANY_COLS) {
-        int64_t n = units >= 384 ? 1 : 512 / units;
-        if (n > (steps + 7) / 8) n = (steps + 7) / 8;
+        // (tiles need not be full: at most this many blocks have columns at all)
+        const int64_t some = Hkv * (n_tiles + n_rows * p.per / MANY_COLS);
+        if (units > some) units = some;
+        int64_t n = units >= 512 ? 1 : units >= 128 ? (512 + units - 1) / units : 512 / units;
+        const int64_t least = units >= 128 ? 16 : 8;                  // steps of a run
+        if (n > (steps + least - 1) / least) n = (steps + least - 1) / least;
         if (n > 1) p.run = (int)((steps + n - 1) / n), p.runs = (int)((steps + p.run - 1) / p.run);
     } else if (n_tiles <= SHARED_TILES && steps > 8) {
         const int64_t fours = (units * steps + 3) / 4;
@@ -564,8 +570,8 @@ bool merged_in_launch(const Plan& p, int Hkv, int n_tiles, int tile_rows) {
     const int64_t cols = (int64_t)tile_rows * p.per, units = (int64_t)n_tiles * Hkv * p.cblocks;
     return (cols < p.cols ? cols : p.cols) * (p.groups / units + 1) < 256;
 }
-int64_t part_floats(const Plan& p, int Hkv, int dim, int n_tiles) {
-    if (p.cols == MANY_COLS) return p.runs > 1 ? (int64_t)n_tiles * Hkv * p.cblocks * p.runs * MANY_COLS * (dim + 2) : 0;
+int64_t part_floats(const Plan& p, int64_t n_rows, int64_t H, int dim, int n_tiles) {
+    if (p.cols == MANY_COLS) return p.runs > 1 ? n_rows * H * p.runs * (dim + 2) : 0;
     return p.groups ? head_floats(n_tiles) + 2 * (int64_t)p.groups * p.cols * (dim + 2) : 0;
 }
 
@@ -616,8 +622,8 @@ int dispatch(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
 PCB_EXPORT int64_t pcb_attn_pages_part(int32_t n_rows, int32_t H, int32_t Hkv, int32_t dim, int32_t n_tiles, int32_t tile_rows, int32_t longest) {
     PCB_REQUIRE(n_rows >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && dim > 0 && n_tiles >= 0 && tile_rows > 0 && longest >= 0, PCB_ERR_ARG, "pcb_attn_pages_part: bad sizes");
     if (n_rows == 0 || n_tiles == 0) return 0;
-    const Plan p = plan_of(H, Hkv, dim, n_tiles, tile_rows, longest);
-    return part_floats(p, Hkv, dim, n_tiles);
+    const Plan p = plan_of(n_rows, H, Hkv, dim, n_tiles, tile_rows, longest);
+    return part_floats(p, n_rows, H, dim, n_tiles);
 }
 
 PCB_EXPORT int pcb_attn_pages(const pcb_attn_pages_args* a, void* stream) {
@@ -635,17 +641,17 @@ PCB_EXPORT int pcb_attn_pages(const pcb_attn_pages_args* a, void* stream) {
                     a->q_head_stride % es == 0 && a->ldo % es == 0 && a->out_head_stride % es == 0,
                 PCB_ERR_ARG, "pcb_attn_pages: rows, heads, codes and tiles start on 16 bytes");
     const int64_t longest = a->longest > 0 ? a->longest : (int64_t)a->max_pages * a->page_size;
-    Plan p = plan_of(a->H, a->Hkv, a->dim, a->n_tiles, a->tile_rows, longest);
+    Plan p = plan_of(a->n_rows, a->H, a->Hkv, a->dim, a->n_tiles, a->tile_rows, longest);
     if (a->window > 0 && (int64_t)a->window + a->tile_rows + 62 < longest) {   // no tile sees more keys than this: fewer runs, never more scratch
-        const Plan w = plan_of(a->H, a->Hkv, a->dim, a->n_tiles, a->tile_rows, (int64_t)a->window + a->tile_rows + 62);
-        if (part_floats(w, a->Hkv, a->dim, a->n_tiles) <= part_floats(p, a->Hkv, a->dim, a->n_tiles)) p = w;
+        const Plan w = plan_of(a->n_rows, a->H, a->Hkv, a->dim, a->n_tiles, a->tile_rows, (int64_t)a->window + a->tile_rows + 62);
+        if (part_floats(w, a->n_rows, a->H, a->dim, a->n_tiles) <= part_floats(p, a->n_rows, a->H, a->dim, a->n_tiles)) p = w;
     }
     p.ps = pcb_log2(a->page_size);
     // (costs are counted in 31 bits; whoever has more of them has enough units)
     if (p.groups && (int64_t)a->n_tiles * a->Hkv * p.cblocks > 0x7fffffff / ((int64_t)a->max_pages * a->page_size / 64 + 2 + UNIT_STEPS) - MAX_GROUPS) p.groups = 0;
     PCB_REQUIRE((int64_t)a->Hkv * p.cblocks <= 65535 && p.per <= 2048 && (int64_t)a->tile_rows * a->H <= 1 << 19 && a->H <= 65535 && a->n_tiles < 1 << 23 && (p.cols != MANY_COLS || (int64_t)a->n_tiles * a->Hkv * p.cblocks < 1 << 23), PCB_ERR_ARG,
                 "pcb_attn_pages: too many tiles, heads or tile rows (heads times tile rows up to 2^19, 2048 query heads a key head)");
-    PCB_REQUIRE((!p.groups && p.runs == 1) || (a->part && (uintptr_t)a->part % 16 == 0 && a->part_floats >= part_floats(p, a->Hkv, a->dim, a->n_tiles)), PCB_ERR_ARG,
+    PCB_REQUIRE((!p.groups && p.runs == 1) || (a->part && (uintptr_t)a->part % 16 == 0 && a->part_floats >= part_floats(p, a->n_rows, a->H, a->dim, a->n_tiles)), PCB_ERR_ARG,
                 "pcb_attn_pages: shared key runs need pcb_attn_pages_part floats");
     PCB_REQUIRE((uintptr_t)a->counters % 4 == 0, PCB_ERR_ARG, "pcb_attn_pages: counters are whole numbers");
     pcb_attn_pages_args b = *a;

@@ -261,10 +261,10 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_p
     if (!live) return;
     l = sum2(l);
     E* op = (E*)a.out + ((int64_t)tl.row0 + qr) * a.ldo + (int64_t)h * a.out_head_stride;
-    const int cc = col - col0;
-    float* pp = a.part + ((((int64_t)t * a.Hkv + hk) * pl.cblocks + cb) * pl.runs + blockIdx.y) * MANY_COLS * (dim + 2);
+    const int64_t at_part = (((int64_t)tl.row0 + qr) * a.H + h) * pl.runs + blockIdx.y;
+    float* pp = a.part + at_part * dim;
     const float f = split ? 1.0f : finished<E>(a, h, M, l, 16384.0f) * (1.0f / 16384.0f);
-    if (split && hh == 0) *reinterpret_cast<float2*>(pp + MANY_COLS * dim + 2 * cc) = float2{M, l};
+    if (split && hh == 0) *reinterpret_cast<float2*>(a.part + (int64_t)a.n_rows * a.H * pl.runs * dim + 2 * at_part) = float2{M, l};
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_p
             const int at = 32 * d + 8 * q + 4 * hh;
             if (at >= dim) continue;
             if (split)
-                *reinterpret_cast<f4*>(pp + cc * dim + at) = f4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+                *reinterpret_cast<f4*>(pp + at) = f4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
             else
                 store4(op + at, o[d][4 * q] * f, o[d][4 * q + 1] * f, o[d][4 * q + 2] * f, o[d][4 * q + 3] * f);
         }
