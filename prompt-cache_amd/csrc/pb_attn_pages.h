@@ -31,6 +31,10 @@ __device__ __forceinline__ int row_of(const Plan& pl, int x) { return pl.per == 
 template <typename E>
 __device__ __forceinline__ float pow_of(float x) { return __builtin_amdgcn_exp2f(sizeof(E) == 4 ? x * LOG2E : x); }
 
+// What a sum of products of a query and a key stands for.  Above 0 and finite whatever the two are (a row of zeros over the smallest scale would give 0, and -infinity, a key that is
+// not seen, times 0 is no number); sums that this changes are 0 or too small to count, or beyond all numbers
+__device__ __forceinline__ float score_unit(float qs, float ks) { return __builtin_fminf(__builtin_fmaxf(qs * ks, 1.17549435e-38f), 3.40282347e38f); }
+
 // e^(x - M) of an fp32 score: 2^(d log2 e) with log2 e in two parts, so that the error does not grow with |d|
 __device__ __forceinline__ float exp_of_score(float x, float M) {
     const float d = __builtin_fmaxf(x - M, -200.0f);

@@ -333,7 +333,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
                         if (!(page >= 0 && key >= lo[n] && key < hi[n])) acc[n][e >> 2][e & 3] = NEG;
                     }
                 }
-                weights<E, PARTS>(acc[n], qs[n] * ks, vs, M[n], l[n], alpha[n], wf[n]);
+                weights<E, PARTS>(acc[n], score_unit(qs[n], ks), vs, M[n], l[n], alpha[n], wf[n]);
             }
             __builtin_amdgcn_sched_barrier(0);
             // values: codes behind the last written key are whatever the memory held, and no number times 0 is 0 for all of them

@@ -201,7 +201,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_p
             float f[4], top = NEG;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                f[q] = qs * ks[q];
+                f[q] = score_unit(qs, ks[q]);
                 float m = acc[q >> 1][8 * (q & 1)];
 #pragma unroll
                 for (int e = 1; e < 8; ++e) m = fmaxf(m, acc[q >> 1][8 * (q & 1) + e]);

@@ -222,6 +222,33 @@ def test_append_with_heads_outside_and_another_stream():
     pool.check()
 
 
+@pytest.mark.parametrize("kind, dtype", [("e4m3", "bf16"), ("int8", "f32")])
+def test_rows_beyond_the_caches(kind, dtype):
+    """Calls of so many rows that these go past the caches store and read what calls of few rows do."""
+    from promptcache_amd import _blocks as B
+    P, Hkv, dim, n = 64, 16, 128, 4300
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    assert n * Hkv * dim * (4 if dtype == "bf16" else 8) > 32 << 20
+    pools = [Pool(n // P + 3, Hkv, P, dim, kind).dev for _ in range(2)]
+    slots = torch.arange(7, 7 + n, dtype=torch.int64, device=DEV)
+    k, v = (rows_of(gen, (n, Hkv, dim), DT[dtype]) for _ in range(2))
+    B.pages_append(k, v, slots, *pools[0])
+    at = 0
+    for m in (57, 1024, 1600, 1619):                                 # (cut where pages end)
+        B.pages_append(k[at:at + m], v[at:at + m], slots[at:at + m], *pools[1])
+        at += m
+    assert at == n and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(*pools))
+    whole, parts = ([torch.zeros_like(k), torch.zeros_like(v)] for _ in range(2))
+    B.pages_read(slots, *pools[0], *whole)
+    for i in range(0, n, 500):
+        B.pages_read(slots[i:i + 500], *pools[0], *(t[i:i + 500] for t in parts))
+    assert torch.equal(whole[0], parts[0]) and torch.equal(whole[1], parts[1])
+    some = np.arange(n - 40, n)
+    for got, codes, scales in ((whole[0], pools[0][0].view(torch.uint8), pools[0][1]), (whole[1], pools[0][2].view(torch.uint8).transpose(2, 3), pools[0][3])):
+        want = O.read(7 + some, codes.cpu().numpy(), scales.cpu().numpy(), P, kind, dim)
+        assert np.array_equal(got[n - 40:].double().cpu().numpy(), want)
+
+
 # ---- attention ----------------------------------------------------------------------------------------------------------------------------
 class Requests:
     """Sequences of given lengths in a pool of written pages (garbage behind them), and queries of their last rows."""
@@ -307,7 +334,10 @@ SIZES = [  # past, new, H, Hkv, dim, P, tile rows
     ([0], [1], 1, 1, 16, 16, 1), ([300, 7, 0, 63, 64, 1000], [1] * 6, 8, 2, 64, 16, 1), ([129, 4, 400], [1, 1, 1], 16, 1, 128, 64, 1), ([70, 1], [1, 1], 20, 1, 80, 32, 1),
     ([500], [1], 6, 2, 256, 128, 1), ([90, 0, 33], [5, 17, 3], 4, 4, 32, 32, 4), ([0, 200], [40, 31], 6, 3, 96, 64, 16), ([0], [130], 5, 5, 128, 128, 128),
     ([1500], [27], 4, 4, 128, 32, 27), ([10, 60, 0, 5], [100, 1, 65, 0], 8, 2, 192, 16, 64), ([3], [70], 10, 2, 48, 16, 128), ([2200, 100], [2, 1], 3, 3, 128, 64, 2),
-    ([0, 77], [9, 260], 7, 1, 64, 16, 100), ([640], [33], 16, 8, 128, 64, 64)]
+    ([0, 77], [9, 260], 7, 1, 64, 16, 100), ([640], [33], 16, 8, 128, 64, 64),
+    # results of many workgroups put together: by the last of them, in a launch of their own, of blocks of 128 columns
+    ([9000], [1], 2, 1, 64, 64, 1), ([5000], [9], 3, 1, 32, 16, 9), ([3000, 2100], [50, 3], 2, 1, 128, 32, 64), ([700], [1], 70, 1, 32, 16, 1), ([2000], [6], 12, 2, 96, 128, 6),
+    ([1800, 30], [1, 1], 5, 5, 192, 16, 1), ([2500], [40], 4, 1, 192, 64, 40), ([1300], [3], 4, 2, 256, 32, 3), ([900], [45], 3, 1, 256, 128, 128)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -399,6 +429,70 @@ def test_attention_of_odd_queries(T, dtype):
     none = torch.isnan(got)
     assert none[7, 1].all() and none[9, 0].all() and int(none.sum()) == 128
     r.check(torch.where(none, r.run(T), got))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("T", [1, 20])
+def test_attention_of_zeros_over_small_keys(T, dtype):
+    """A row of zeros sees all its keys alike, however small their scales, and none of those it does not see."""
+    r = Requests([70], [20], 4, 2, 64, 16, "int8", dtype, seed=8, scales=(-2, 1))
+    r.q[3:7] = 0
+    r.q[7] *= 1e-35
+    r.ks[:] = 2.0 ** -40
+    for scale in (1.0, 1e-3, 1e-20):
+        r.check(r.run(T, scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("T", [1, 9, 64])
+def test_attention_many_times_alike(T):
+    """The same call again and again, among others, on two streams at once: the same bits each time."""
+    a, b = (Requests([4000, 77, 900], [T, T, T], 8, 2, 128, 64, "e4m3", "bf16", seed=s) for s in (1, 2))
+    want = [r.run(T) for r in (a, b)]
+    a.check(want[0])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    from promptcache_amd import _blocks as B
+    args = []
+    for r in (a, b):
+        args.append((r.q, torch.tensor(r.tiles(T), dtype=torch.int32, device=DEV), T, i32(r.kv), *r.device()))
+    torch.cuda.synchronize()
+    outs = [[torch.zeros_like(r.q) for _ in range(40)] for r in (a, b)]
+    for i in range(40):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                B.attn_pages(*args[k], outs[k][i], scale=1.0)
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(o, want[k]) for o in outs[k])
+
+
+def test_attention_in_a_graph_is_the_eager_one_but_for_its_merge():
+    """A captured call merges in a launch of its own: the same sums in the same order of runs, off by roundings of fp32."""
+    r = Requests([4000, 700], [1, 1], 8, 2, 128, 64, "e4m3", "f32", seed=3)
+    from promptcache_amd import _blocks as B
+    eager = r.run(1)
+    r.check(eager)
+    tiles, kv, dev = torch.tensor(r.tiles(1), dtype=torch.int32, device=DEV), i32(r.kv), r.device()
+    floats = B.attn_pages_part(2, 8, 2, 128, 2, 1, 4001)
+    part, out = torch.zeros(floats, device=DEV), torch.zeros_like(r.q)
+    torch.cuda.synchronize()
+    g, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=st):
+        B.attn_pages(r.q, tiles, 1, kv, *dev, out, scale=1.0, longest=4001, part=part)
+    for _ in range(4):
+        out.zero_()
+        g.replay()
+        r.run(1)
+        torch.cuda.synchronize()
+        r.check(out)
+
+
+def test_attention_of_more_tiles_than_are_shared_out():
+    """Over 512 tiles: a workgroup a unit."""
+    n = 600
+    rng = np.random.default_rng(4)
+    r = Requests([int(v) for v in rng.integers(0, 40, n)], [1] * n, 4, 2, 32, 16, "int8", "bf16", seed=5)
+    r.check(r.run(1))
+    r.check(r.run(1, longest=5000))
 
 
 def test_attention_with_a_head_of_a_wrong_bound():
