@@ -68,7 +68,7 @@ __device__ __forceinline__ Tile tile_of(const pcb_attn_pages_args& a, int t, int
     Tile x;
     x.seq = r.x, x.pos = r.y, x.rows = r.z < a.tile_rows ? r.z : a.tile_rows, x.row0 = r.w;
     x.kv = 0, x.s0 = 0, x.s1 = 0;
-    if (r.x < 0 || r.x >= a.n_seqs || r.y < 0 || r.w < 0 || x.rows <= 0 || (int64_t)r.w + x.rows > a.n_rows) {
+    if (r.x < 0 || r.x >= a.n_seqs || r.y < 0 || r.w < 0 || x.rows <= 0 || r.y > 0x7fffffff - x.rows || (int64_t)r.w + x.rows > a.n_rows) {
         x.rows = 0;
         return x;
     }

@@ -575,6 +575,11 @@ int64_t part_floats(const Plan& p, int64_t n_rows, int64_t H, int dim, int n_til
     return p.groups ? head_floats(n_tiles) + 2 * (int64_t)p.groups * p.cols * (dim + 2) : 0;
 }
 
+// sizes for which a call's counts below stay inside their types
+bool sizes_ok(int64_t H, int64_t Hkv, int64_t n_tiles, int64_t tile_rows) {
+    return H > 0 && H <= 65535 && Hkv > 0 && H % Hkv == 0 && H / Hkv <= 2048 && n_tiles >= 0 && n_tiles < 1 << 23 && tile_rows > 0 && tile_rows * H <= 1 << 19;
+}
+
 template <typename E, int CODE, int DB>
 void launch_rows(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
     const dim3 grid(pl.groups ? pl.groups : a.n_tiles, pl.groups ? 1 : a.Hkv * pl.cblocks), block(256);
@@ -586,11 +591,18 @@ void launch_rows(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t strea
     hipLaunchKernelGGL((attn_pages_rows_kernel<E, CODE, DB, 1>), grid, block, 0, stream, a, pl);
 }
 
+int merge_sets(const pcb_attn_pages_args& a, const Plan& pl) {
+    const int64_t units = (int64_t)a.n_tiles * a.Hkv * pl.cblocks, results = pl.cols == MANY_COLS ? pl.runs : pl.groups / units + 1;
+    return results > 32 ? 16 : results > 16 ? 8 : results > 8 ? 4 : results > 4 ? 2 : 1;
+}
+int64_t merge_groups(const pcb_attn_pages_args& a, const Plan& pl) {
+    const int wide = 16 / merge_sets(a, pl);
+    return a.n_tiles * (((int64_t)a.tile_rows * a.H + wide - 1) / wide);
+}
 template <typename E, int DB>
 void launch_merge(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
-    const int64_t units = (int64_t)a.n_tiles * a.Hkv * pl.cblocks, results = pl.cols == MANY_COLS ? pl.runs : pl.groups / units + 1;
-    const int sets = results > 32 ? 16 : results > 16 ? 8 : results > 8 ? 4 : results > 4 ? 2 : 1, wide = 16 / sets;
-    hipLaunchKernelGGL((attn_pages_merge_kernel<E, DB>), dim3((unsigned)(a.n_tiles * (((int64_t)a.tile_rows * a.H + wide - 1) / wide))), dim3(256), 0, stream, a, pl, sets);
+    const int sets = merge_sets(a, pl);
+    hipLaunchKernelGGL((attn_pages_merge_kernel<E, DB>), dim3((unsigned)merge_groups(a, pl)), dim3(256), 0, stream, a, pl, sets);
 }
 
 template <typename E, int CODE>
@@ -620,7 +632,7 @@ int dispatch(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
 }  // namespace
 
 PCB_EXPORT int64_t pcb_attn_pages_part(int32_t n_rows, int32_t H, int32_t Hkv, int32_t dim, int32_t n_tiles, int32_t tile_rows, int32_t longest) {
-    PCB_REQUIRE(n_rows >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && dim > 0 && n_tiles >= 0 && tile_rows > 0 && longest >= 0, PCB_ERR_ARG, "pcb_attn_pages_part: bad sizes");
+    PCB_REQUIRE(n_rows >= 0 && dim > 0 && dim <= 256 && longest >= 0 && sizes_ok(H, Hkv, n_tiles, tile_rows), PCB_ERR_ARG, "pcb_attn_pages_part: bad sizes");
     if (n_rows == 0 || n_tiles == 0) return 0;
     const Plan p = plan_of(n_rows, H, Hkv, dim, n_tiles, tile_rows, longest);
     return part_floats(p, n_rows, H, dim, n_tiles);
@@ -640,6 +652,9 @@ PCB_EXPORT int pcb_attn_pages(const pcb_attn_pages_args* a, void* stream) {
     PCB_REQUIRE(((uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->kcodes | (uintptr_t)a->vcodes | (uintptr_t)a->tiles) % 16 == 0 && a->ldq % es == 0 &&
                     a->q_head_stride % es == 0 && a->ldo % es == 0 && a->out_head_stride % es == 0,
                 PCB_ERR_ARG, "pcb_attn_pages: rows, heads, codes and tiles start on 16 bytes");
+    PCB_REQUIRE((a->ldo != 0 || a->n_rows == 1) && (a->out_head_stride != 0 || a->H == 1), PCB_ERR_ARG, "pcb_attn_pages: results have places of their own");
+    PCB_REQUIRE(sizes_ok(a->H, a->Hkv, a->n_tiles, a->tile_rows), PCB_ERR_ARG,
+                "pcb_attn_pages: too many tiles, heads or tile rows (heads times tile rows up to 2^19, 2048 query heads a key head)");
     const int64_t longest = a->longest > 0 ? a->longest : (int64_t)a->max_pages * a->page_size;
     Plan p = plan_of(a->n_rows, a->H, a->Hkv, a->dim, a->n_tiles, a->tile_rows, longest);
     if (a->window > 0 && (int64_t)a->window + a->tile_rows + 62 < longest) {   // no tile sees more keys than this: fewer runs, never more scratch
@@ -649,8 +664,10 @@ PCB_EXPORT int pcb_attn_pages(const pcb_attn_pages_args* a, void* stream) {
     p.ps = pcb_log2(a->page_size);
     // (costs are counted in 31 bits; whoever has more of them has enough units)
     if (p.groups && (int64_t)a->n_tiles * a->Hkv * p.cblocks > 0x7fffffff / ((int64_t)a->max_pages * a->page_size / 64 + 2 + UNIT_STEPS) - MAX_GROUPS) p.groups = 0;
-    PCB_REQUIRE((int64_t)a->Hkv * p.cblocks <= 65535 && p.per <= 2048 && (int64_t)a->tile_rows * a->H <= 1 << 19 && a->H <= 65535 && a->n_tiles < 1 << 23 && (p.cols != MANY_COLS || (int64_t)a->n_tiles * a->Hkv * p.cblocks < 1 << 23), PCB_ERR_ARG,
-                "pcb_attn_pages: too many tiles, heads or tile rows (heads times tile rows up to 2^19, 2048 query heads a key head)");
+    // (a grid is less than 2^32 threads)
+    PCB_REQUIRE((int64_t)a->Hkv * p.cblocks <= 65535 && (p.cols != MANY_COLS || (int64_t)a->n_tiles * a->Hkv * p.cblocks < 1 << 23) &&
+                    ((!p.groups && p.runs == 1) || merge_groups(*a, p) < 1 << 24),
+                PCB_ERR_ARG, "pcb_attn_pages: too many tiles of too many heads and rows");
     PCB_REQUIRE((!p.groups && p.runs == 1) || (a->part && (uintptr_t)a->part % 16 == 0 && a->part_floats >= part_floats(p, a->n_rows, a->H, a->dim, a->n_tiles)), PCB_ERR_ARG,
                 "pcb_attn_pages: shared key runs need pcb_attn_pages_part floats");
     PCB_REQUIRE((uintptr_t)a->counters % 4 == 0, PCB_ERR_ARG, "pcb_attn_pages: counters are whole numbers");

@@ -493,9 +493,9 @@ int check_rows(const pcb_pages_rows_args* a, const char* who) {
 
 PCB_EXPORT int pcb_page_tables(const pcb_page_tables_args* a, void* stream) {
     PCB_REQUIRE(a && a->struct_bytes == sizeof(pcb_page_tables_args), PCB_ERR_ARG, "pcb_page_tables: struct size mismatch");
-    PCB_REQUIRE(a->n_seqs > 0 && a->max_pages > 0 && a->ld_table >= a->max_pages && pcb_page_size_ok(a->page_size) && a->n_rows >= 0 && (int64_t)a->n_seqs * a->max_pages < 0x7fffffff &&
-                    (int64_t)a->max_pages * a->page_size <= 0x7fffffff,
-                PCB_ERR_ARG, "pcb_page_tables: bad sizes (pages of 16, 32, 64 or 128 tokens, positions of 31 bits)");
+    PCB_REQUIRE(a->n_seqs > 0 && a->max_pages > 0 && a->ld_table >= a->max_pages && pcb_page_size_ok(a->page_size) && a->n_rows >= 0 && a->n_rows <= 1 << 30 &&
+                    (int64_t)a->n_seqs * a->max_pages < 0x7fffffff && (int64_t)a->max_pages * a->page_size <= 0x7fffffff,
+                PCB_ERR_ARG, "pcb_page_tables: bad sizes (pages of 16, 32, 64 or 128 tokens, positions of 31 bits, up to 2^30 rows)");
     PCB_REQUIRE(a->cached && a->brings && a->table && (a->row_slot || a->n_rows == 0), PCB_ERR_ARG, "pcb_page_tables: null pointer");
     PCB_REQUIRE(!a->ring || (a->ring_cap > 0 && a->ring_state && a->ring_out), PCB_ERR_ARG, "pcb_page_tables: a ring comes with its state, and a place for the new one");
     PCB_REQUIRE(!a->tiles || (a->tile_rows > 0 && (uintptr_t)a->tiles % 16 == 0 && a->n_tiles >= (int64_t)a->n_seqs + a->n_rows / a->tile_rows), PCB_ERR_ARG,
@@ -560,6 +560,8 @@ PCB_EXPORT int pcb_pages_append(const pcb_pages_rows_args* a, void* stream) {
 PCB_EXPORT int pcb_pages_read(const pcb_pages_rows_args* a, void* stream) {
     const int rc = check_rows(a, "pcb_pages_read");
     if (rc != PCB_OK || a->n_rows == 0) return rc;
+    PCB_REQUIRE(((a->ldk != 0 && a->ldv != 0) || a->n_rows == 1) && ((a->k_head_stride != 0 && a->v_head_stride != 0) || a->Hkv == 1), PCB_ERR_ARG,
+                "pcb_pages_read: results have places of their own");
     const RowsView v{a->row_slot, a->n_rows, pcb_log2(a->page_size), (int64_t)a->n_pages * a->page_size};
     const int win = window(a->n_rows, a->Hkv, 4, 32);
     const int64_t waves = ((int64_t)a->n_rows + win - 1) / win * a->Hkv;

@@ -81,7 +81,7 @@ def attn_args(**kw):
     ("pcb_page_tables", tables_args, b) for b in (
         dict(struct_bytes=8), dict(n_seqs=0), dict(max_pages=0), dict(ld_table=4), dict(page_size=48), dict(page_size=8), dict(page_size=256), dict(n_rows=-1), dict(cached=None),
         dict(brings=None), dict(table=None), dict(row_slot=None), dict(ring_cap=0), dict(ring_state=None), dict(ring_out=None), dict(tile_rows=0), dict(tiles=PTR + 4),
-        dict(n_tiles=5), dict(n_seqs=1 << 20, max_pages=1 << 12, ld_table=1 << 12), dict(n_seqs=1, max_pages=1 << 27, ld_table=1 << 27))
+        dict(n_rows=(1 << 30) + 1, n_tiles=1 << 29), dict(n_tiles=5), dict(n_seqs=1 << 20, max_pages=1 << 12, ld_table=1 << 12), dict(n_seqs=1, max_pages=1 << 27, ld_table=1 << 27))
 ] + [
     (entry, rows_args, b) for entry in ("pcb_pages_append", "pcb_pages_read") for b in (
         dict(struct_bytes=8), dict(dtype=2), dict(code=2), dict(n_rows=-1), dict(n_pages=0), dict(page_size=24), dict(Hkv=0), dict(dim=0), dict(dim=24), dict(dim=272), dict(k=None),
@@ -93,7 +93,11 @@ def attn_args(**kw):
         dict(page_size=17), dict(H=5), dict(Hkv=0), dict(dim=40), dict(dim=512), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(longest=-1),
         dict(q=None), dict(tiles=None), dict(kv_len=None), dict(table=None), dict(kcodes=None), dict(vscale=None), dict(out=None), dict(q=PTR + 2), dict(out=PTR + 8), dict(tiles=PTR + 4),
         dict(ldq=129), dict(out_head_stride=33), dict(longest=1 << 20), dict(longest=1 << 20, part=PTR, part_floats=100), dict(longest=1 << 20, part=PTR + 4, part_floats=1 << 40),
-        dict(tile_rows=1 << 22), dict(max_pages=1 << 27, ld_table=1 << 27))
+        dict(tile_rows=1 << 22), dict(max_pages=1 << 27, ld_table=1 << 27), dict(ldo=0), dict(out_head_stride=0), dict(n_tiles=1 << 23),
+        dict(n_tiles=1 << 30, H=1 << 30, Hkv=1 << 30), dict(H=4098, Hkv=2), dict(H=65536, Hkv=2048),
+        dict(n_tiles=512, tile_rows=8, H=65535, Hkv=65535, longest=1000, part=PTR, part_floats=1 << 50))
+] + [
+    ("pcb_pages_read", rows_args, b) for b in (dict(ldk=0), dict(ldv=0), dict(k_head_stride=0), dict(v_head_stride=0))
 ])
 def test_what_is_refused(entry, make, bad):
     lib = B.load()
@@ -113,8 +117,9 @@ def test_scratch_of_key_runs():
     one = B.attn_pages_part(1, 32, 8, 128, 1, 1, 100000)
     assert one > 0
     assert B.attn_pages_part(0, 32, 8, 128, 0, 1, 100000) == 0
-    with pytest.raises(RuntimeError):
-        B.attn_pages_part(1, 32, 7, 128, 1, 1, 100)
+    for bad in ((1, 32, 7, 128, 1, 1, 100), (1, 1 << 30, 1 << 30, 128, 1 << 30, 1, 1 << 20), (1, 32, 8, 272, 1, 1, 100), (1, 32, 8, 128, 1, 0, 100), (1, 32, 8, 128, 1 << 23, 1, 100)):
+        with pytest.raises(RuntimeError):
+            B.attn_pages_part(*bad)
 
 
 def test_wrappers_name_what_is_wrong():
