@@ -490,7 +490,7 @@ class PageCache:
         s.tiles = self._buf("tiles", (self.seqs + rows // tile_rows, 4), torch.int32)
         B.page_tables(self.cached, brings, self.table, self.page_size, row_slot=s.row_slot, kv_len=self.cached, row_start=s.row_start, row_seq=s.row_seq, row_pos=s.row_pos,
                       tiles=s.tiles, tile_rows=tile_rows, status=s.status, ring=self.ring, ring_state=self.ring_state, ring_out=self.ring_state, keep=self.keep)
-        if self._shared:
+        if self._shared or self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():   # (a replay may follow a later `share`)
             self.keep.masked_fill_(brings < 0, 0)                 # (whoever takes the sequence's place owns all of its pages)
         s.kv_len = self.cached
         return s

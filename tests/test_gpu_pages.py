@@ -431,6 +431,27 @@ def test_attention_of_odd_queries(T, dtype):
     r.check(torch.where(none, r.run(T), got))
 
 
+@pytest.mark.parametrize("T", [1, 4, 32])
+def test_attention_passes_over_tiles_that_are_none(T):
+    """Tiles of no sequence, before the first position, of no rows, out of the rows or behind the last position that there can be."""
+    r = Requests([700, 40], [33, 2], 4, 2, 64, 32, "e4m3", "bf16", seed=9)
+    top = 2 ** 31 - 1
+    none = [[-1, 0, 1, 0], [2, 0, 1, 0], [0, -1, 1, 0], [0, 5, 0, 0], [0, 5, -3, 0], [0, 5, 1, 35], [0, 5, 1, -1], [0, 5, 1, top], [top, top, top, top], [0, top, 1, 0], [1, top - T + 1, T, 0]]
+    want = r.run(T)
+    for window in (0, 30):
+        got = r.run(T, window=window, tiles=none)
+        assert bool((got == 55).all())
+    assert torch.equal(want, r.run(T, tiles=none[:5] + r.tiles(T) + none[5:]))
+
+
+@pytest.mark.parametrize("T", [1, 9, 64])
+def test_attention_in_place(T):
+    """Results may take their queries' place."""
+    r = Requests([4000, 77, 900], [T, T, T], 8, 2, 128, 64, "e4m3", "bf16", seed=3)
+    want, q = r.run(T), r.q.clone()
+    assert torch.equal(r.run(T, q=q, out=q), want)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("T", [1, 20])
 def test_attention_of_zeros_over_small_keys(T, dtype):
@@ -652,3 +673,29 @@ def test_a_captured_step_moves_on_by_itself():
     assert caches[0].cached.tolist() == [71, 56, 42, 81, 45]
     for a, b in zip((caches[0].kcodes[0], caches[0].vcodes[0], caches[0].kscale[0]), (caches[1].kcodes[0], caches[1].vcodes[0], caches[1].kscale[0])):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_a_captured_step_gives_back_what_a_later_share_left_it():
+    """A graph captured before the first shared prefix: a sequence that is over keeps the shared pages out of the ring once, and its place's next one gives back all of its own."""
+    from promptcache_amd.model.kv_arena import PageCache
+    cache = PageCache([(1, 16)], 2, 10, DEV, page_size=16)
+    brings = torch.zeros(2, dtype=torch.int32, device=DEV)
+    cache.begin(brings, 40)
+    torch.cuda.synchronize()
+    graph, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=st):
+        cache.begin(brings, 40)
+
+    def step(*b):
+        brings.copy_(torch.tensor(b, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        return cache.ring_state.tolist()[1]
+
+    assert step(40, 0) == 7
+    cache.share(0, 1, 32)
+    assert step(0, 20) == 5
+    assert step(0, -1) == 7
+    assert step(0, 40) == 4
+    assert step(0, -1) == 7
+    assert step(-1, 0) == 10 and sorted(cache.ring.tolist()) == list(range(10))
