@@ -26,49 +26,42 @@ __device__ __forceinline__ float sum4(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 
-// The lane's part of a query row: sixteen neighbouring elements for each 64, as they are in memory
-template <typename E, int DB>
+// Sixteen neighbouring elements of a query row, as they are in memory
+template <typename E>
 struct Query {
-    u32x4 w[DB][sizeof(E)];
-};
-template <typename E, int DB>
-__device__ __forceinline__ void load_query(Query<E, DB>& q, const E* p, int dim, int g) {
-#pragma unroll
-    for (int c = 0; c < DB; ++c)
-#pragma unroll
-        for (int k = 0; k < (int)sizeof(E); ++k) q.w[c][k] = *reinterpret_cast<const u32x4*>(p + min(64 * c + 16 * g, dim - 16) + k * (16 / sizeof(E)));
-}
-// .. as operands, two k-steps of 32 for each 64 elements, zeros behind the row's end and where the column is nobody's.  -> the power of two that the row was divided by: its largest
-// element becomes 2^14 .. 2^15, and what is 2^-28 of that is still a normal half
-template <typename E, int DB, int PARTS>
-__device__ __forceinline__ float operands(const Query<E, DB>& q, int dim, int g, bool live, h8 (&qf)[PARTS][2 * DB]) {
-    auto at = [&](int c, int e) {
-        float x;
+    u32x4 w[sizeof(E)];
+    __device__ __forceinline__ float at(int e) const {
         if constexpr (sizeof(E) == 2)
-            x = __uint_as_float(e & 1 ? q.w[c][e >> 3][(e & 7) >> 1] & 0xffff0000u : q.w[c][e >> 3][(e & 7) >> 1] << 16);
+            return __uint_as_float(e & 1 ? w[e >> 3][(e & 7) >> 1] & 0xffff0000u : w[e >> 3][(e & 7) >> 1] << 16);
         else
-            x = __uint_as_float(q.w[c][e >> 2][e & 3]);
-        return live && 64 * c + 16 * g < dim ? x : 0.0f;
-    };
+            return __uint_as_float(w[e >> 2][e & 3]);
+    }
+};
+// .. as halves (PARTS = 2: sums of two) at `to`, the second ones `parts` behind.  THREADS neighbouring lanes hold a row.  -> the power of two that the row was divided by: its largest
+// element becomes 2^14 .. 2^15, and what is 2^-28 of that is still a normal half
+template <typename E, int PARTS, int THREADS>
+__device__ __forceinline__ float as_halves(const Query<E>& q, _Float16* to, int parts) {
     float m = 0.0f;
 #pragma unroll
-    for (int c = 0; c < DB; ++c)
+    for (int e = 0; e < 16; ++e) m = fmaxf(m, __builtin_fabsf(q.at(e)) < __builtin_inff() ? __builtin_fabsf(q.at(e)) : 0.0f);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) m = fmaxf(m, __builtin_fabsf(at(c, e)) < __builtin_inff() ? __builtin_fabsf(at(c, e)) : 0.0f);
-    m = max4(m);
+    for (int o = 1; o < THREADS; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     int e2 = (int)(__float_as_uint(m) >> 23) - 127 - 14;
     e2 = e2 < -110 ? -110 : e2;
-    const float inv = __uint_as_float((uint32_t)(127 - e2) << 23), unit = __uint_as_float((uint32_t)(127 + e2) << 23);
+    const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
 #pragma unroll
-    for (int c = 0; c < DB; ++c)
+    for (int k = 0; k < 2; ++k) {
+        h8 hi, lo;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const float y = at(c, e) * inv;
-            const _Float16 hi = (_Float16)y;
-            qf[0][2 * c + (e >> 3)][e & 7] = hi;
-            if constexpr (PARTS == 2) qf[1][2 * c + (e >> 3)][e & 7] = __builtin_fabsf(y) < __builtin_inff() ? (_Float16)(y - (float)hi) : (_Float16)0.0f;
+        for (int e = 0; e < 8; ++e) {
+            const float y = q.at(8 * k + e) * inv;
+            hi[e] = (_Float16)y;
+            if constexpr (PARTS == 2) lo[e] = __builtin_fabsf(y) < __builtin_inff() ? (_Float16)(y - (float)hi[e]) : (_Float16)0.0f;
         }
-    return unit;
+        *reinterpret_cast<h8*>(to + 8 * k) = hi;
+        if constexpr (PARTS == 2) *reinterpret_cast<h8*>(to + parts + 8 * k) = lo;
+    }
+    return __uint_as_float((uint32_t)(127 + e2) << 23);
 }
 
 // Sixteen scores of a lane (in units of 1 / f; -infinity: not seen) as weights of the second product: w = e^(s - M) vs 2^14 with M the running maximum of s + ln vs over the
@@ -138,10 +131,14 @@ template <typename E, int CODE, int DB, int NC>
 __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_args a, Plan pl) {
     constexpr bool F32 = sizeof(E) == 4;
     constexpr int NW = 4, NT = 256, PARTS = F32 ? 2 : 1, NB = 4 * DB, COLS = 16 * NC;   // NB: value column blocks of 16
+    constexpr int TPC = DB == 1 ? 4 : DB == 2 ? 8 : 16, QLD = 64 * DB + 8;            // threads that bring a query row, and a row of halves
+    static_assert(COLS * TPC <= NT && COLS * QLD * PARTS * 2 <= NW * 16 * (64 * DB + 4) * 4, "a pass, in the results' place");
     __shared__ __attribute__((aligned(16))) float Os[NW][16][64 * DB + 4];
+    _Float16* const Qs = reinterpret_cast<_Float16*>(&Os[0][0][0]);  // (before there are results)
     __shared__ float Ms[NW][COLS], Ls[NW][COLS];
     __shared__ __attribute__((aligned(16))) int4 tiles_s[SHARED_TILES];
-    __shared__ int starts[SHARED_TILES + 1], kv_s[SHARED_TILES], wsum[NW], last_s;
+    __shared__ int starts[SHARED_TILES + 1], kv_s[SHARED_TILES], wsum[NW], found_s, last_s;
+    __shared__ float unit_s[COLS];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int per = pl.per, dim = a.dim, ps = pl.ps, P = 1 << ps;
     const int64_t plane = (int64_t)P * dim;
@@ -194,15 +191,10 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
         int t, j, from, steps, n_steps, mine = 1, g0 = 0, parts = 1, second = 0;  // unit j of tile t, its steps from .. from + n_steps - 1; the workgroups that share it are g0 ..
         Tile tl;
         if (pl.groups) {
-            int lo = 0, hi = a.n_tiles;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (starts[mid] <= at)
-                    lo = mid;
-                else
-                    hi = mid;
-            }
-            t = __builtin_amdgcn_readfirstlane(lo);
+            for (int i = threadIdx.x; i < a.n_tiles; i += NT)
+                if (starts[i] <= at && at < starts[i + 1]) found_s = i;
+            __syncthreads();
+            t = __builtin_amdgcn_readfirstlane(found_s);
             const int4 rec = tiles_s[t];
             tl.seq = __builtin_amdgcn_readfirstlane(rec.x), tl.pos = __builtin_amdgcn_readfirstlane(rec.y), tl.rows = __builtin_amdgcn_readfirstlane(rec.z);
             tl.row0 = __builtin_amdgcn_readfirstlane(rec.w), tl.kv = __builtin_amdgcn_readfirstlane(kv_s[t]);
@@ -266,26 +258,39 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
 #pragma unroll
             for (int b = 0; b < NB; ++b) vr[b] = *reinterpret_cast<const u32x4*>(p + 16 * min(b, last_b) * P);
         };
-        // (the queries are asked for first: loads arrive in order, and they are made operands while the first keys are under way)
-        Query<E, DB> raw[NC];
+        // The queries are asked for first, sixteen elements a thread: loads arrive in order, and they are made halves while the first keys are under way, once for all waves.  (Every
+        // wave its own operands instead: 500 instructions more for each 16 columns before the first product, 27 rows of 32 heads over 8 274 keys 29.6 -> 33.6 us.)
+        const int qc = tid / TPC, qk = tid % TPC;
+        Query<E> raw;
 #pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            const int col = min(col0 + 16 * n + c, rows * per - 1), qr = row_of(pl, col), h = hk * per + col - qr * per;
-            load_query<E, DB>(raw[n], (const E*)a.q + ((int64_t)tl.row0 + qr) * a.ldq + (int64_t)h * a.q_head_stride, dim, g);
+        for (int k = 0; k < (int)sizeof(E); ++k) raw.w[k] = u32x4{0, 0, 0, 0};   // (behind a row's end, and where the column is nobody's)
+        if (col0 + qc <= last_col && qk <= last_b && qc < COLS) {
+            const int col = col0 + qc, qr = row_of(pl, col), h = hk * per + col - qr * per;
+            const E* q = (const E*)a.q + ((int64_t)tl.row0 + qr) * a.ldq + (int64_t)h * a.q_head_stride + 16 * qk;
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(E); ++k) raw.w[k] = *reinterpret_cast<const u32x4*>(q + k * (16 / sizeof(E)));
         }
         int s = s0 + wave, i = 0;
         if (s < s1) {
             look(s);
             fetch_k(s, 0);
         }
+        if (qc < COLS && qk < 4 * DB) {
+            const float unit2 = as_halves<E, PARTS, TPC>(raw, Qs + qc * QLD + 16 * qk, COLS * QLD);
+            if (qk == 0) unit_s[qc] = F32 ? unit2 * a.scale : unit2 * (a.scale * LOG2E);   // bf16: scores in units of ln 2
+        }
+        __syncthreads();
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
             const int col = col0 + 16 * n + c;
             const bool live = col < rows * per;
             const int pos = live ? tl.pos + row_of(pl, col) : -1;
             lo[n] = a.window > 0 ? pos - a.window + 1 : 0, hi[n] = min(kv, pos + 1);
-            const float unit2 = operands<E, DB, PARTS>(raw[n], dim, g, live, qf[n]);
-            qs[n] = F32 ? unit2 * a.scale : unit2 * (a.scale * LOG2E);  // bf16: scores in units of ln 2
+            qs[n] = unit_s[16 * n + c];
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                for (int k = 0; k < 2 * DB; ++k) qf[n][p][k] = *reinterpret_cast<const h8*>(Qs + (p * COLS + 16 * n + c) * QLD + 64 * (k >> 1) + 16 * g + 8 * (k & 1));
         }
         float M[NC], l[NC];
         f4 o[NC][NB];
