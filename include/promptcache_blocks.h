@@ -942,10 +942,10 @@ int pcb_pages_read(const pcb_pages_rows_args* a, void* stream);
  * sequence iff j <= i, j < kv_len[sequence], window <= 0 or i - j < window, and table[sequence][j / P] is a page of the pool.
  *   out = sum_j e^(scale q.k_j) v_j / (sum_j e^(scale q.k_j) + e^sink[h]),   sink (fp32 [H]) optional; a row that sees nothing: 0
  * out may be q, with q's strides.  Query head h reads key head h / (H / Hkv).  scale > 0.  Tiles without rows or of no sequence, and rows outside [0, n_rows), are passed over.
- * longest: an upper bound of kv_len that the host knows (0: max_pages * P, which pcb_attn_pages_part is then given); it decides the number of key runs that workgroups of their own take, whose
- * results need part: pcb_attn_pages_part(...) floats, aligned to 16 bytes.  counters (int32 [512], optional): zero before the first launch that is given them and left zero
- * by every launch; with them a tile of few columns is merged by the last of its workgroups, without them (and tiles of many) in a second launch.  Launches that may run at
- * the same time need a part and counters of their own. */
+ * longest: an upper bound of kv_len that the host knows (0: max_pages * P, which pcb_attn_pages_part is then given); it decides into how many key runs a tile is
+ * cut, whose results need part: pcb_attn_pages_part(...) floats, aligned to 16 bytes.  counters (int32 [512], optional): zero before the first launch that is given them and
+ * left zero by every launch; with them the runs of few columns, where they are few, are merged by the last of their workgroups; without them, and all others, in a second launch.
+ * Launches that may run at the same time need a part and counters of their own.  Up to 65 535 heads, 2 048 of them a key head, 2^23 tiles, heads times tile rows up to 2^19. */
 typedef struct pcb_attn_pages_args {
     uint32_t struct_bytes;
     int32_t dtype, code;

@@ -35,12 +35,18 @@ __device__ __forceinline__ float pow_of(float x) { return __builtin_amdgcn_exp2f
 // not seen, times 0 is no number); sums that this changes are 0 or too small to count, or beyond all numbers
 __device__ __forceinline__ float score_unit(float qs, float ks) { return __builtin_fminf(__builtin_fmaxf(qs * ks, 1.17549435e-38f), 3.40282347e38f); }
 
-// e^(x - M) of an fp32 score: 2^(d log2 e) with log2 e in two parts, so that the error does not grow with |d|
-__device__ __forceinline__ float exp_of_score(float x, float M) {
-    const float d = __builtin_fmaxf(x - M, -200.0f);
-    const float p = d * 1.44269502e+00f, rest = __builtin_fmaf(d, 1.92596303e-08f, __builtin_fmaf(d, 1.44269502e+00f, -p));
-    const float q = __builtin_amdgcn_exp2f(p);
-    return x == NEG ? 0.0f : x == x ? __builtin_fmaf(q, rest * 6.93147182e-01f, q) : x;
+// e^(x - M) of an fp32 score x = s f: 2^p e^(d - p ln 2) with p = d log2 e as it was rounded, so that the error does not grow with |d| by more than 2^-28 of it.  What is no number
+// comes out as one (or_not)
+__device__ __forceinline__ float exp_of_score(float s, float f, float M) {
+    const float d = __builtin_fmaxf(__builtin_fmaf(s, f, -M), -200.0f), p = d * 1.44269502e+00f, q = __builtin_amdgcn_exp2f(p);
+    return __builtin_fmaf(q, __builtin_fmaf(p, -6.93147182e-01f, d), q);
+}
+// A sum of scores is no number if one of them is none (or some are infinite and some -infinity, whose exponentials have no sum either): a step's sum of exponentials then
+__device__ __forceinline__ float or_not(float sum, float scores) { return scores == scores ? sum : scores; }
+// a weight as two halves
+__device__ __forceinline__ void two_halves(float w, _Float16& hi, _Float16& lo) {
+    hi = (_Float16)w;
+    lo = (_Float16)__builtin_fmaf((float)hi, -1.0f, w);
 }
 
 // the quotient of a column: its sums under the maximum m, and the sink.  No score above -infinity: 0, but scores that are no numbers stay so

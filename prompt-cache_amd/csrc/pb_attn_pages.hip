@@ -10,6 +10,10 @@
 // A step walks 64 keys.  Lane group g (16 lanes) owns the sixteen keys 16 g .. 16 g + 15 of the step, in every role: which key a row of the first product's operand is may
 // be chosen freely, so row 4 g + r of its block b is key 16 g + 4 b + r, and the lane's scores are then, in order, the keys of its operand of the second product, sixteen
 // neighbouring codes of a value column, one 16-byte load.  Pages have at least 16 tokens: a lane needs one page number and one pair of scales a step.
+//
+// Bound by the codes' bytes, which are read once, and before them by a chain of loads that each need the one before (tile, length, page number, keys: ~6 us of a launch).  Measured
+// (the launch alone; bf16, 4 heads a key head of 128): 64 single tokens over up to 8 192 keys, 189 MB, 38.6 us = 4.9 TB/s; one over 131 072, 268 MB, 46 us = 5.8 TB/s, 7 more its
+// merge; 27 rows over 8 247 keys of 32 heads, 68 MB, 26.5 us and 5.3: a wave has two steps of its own there.  A copy reaches 4.9 TB/s, a reading stream ~5.9.
 #include "pb_attn_pages.h"
 
 namespace {
@@ -89,15 +93,17 @@ __device__ __forceinline__ void weights(f4 (&acc)[4], float f, float vs, float& 
         sum *= inv_pow2(vs) * (1.0f / 16384.0f);
     } else {
         const float up = vs * 16384.0f;
+        float scores = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float e = exp_of_score(acc[i >> 2][i & 3] * f, M_use);
+            const float e = exp_of_score(acc[i >> 2][i & 3], f, M_use);
+            scores += acc[i >> 2][i & 3];
             sum += e;
-            const float w = e * up;
-            const _Float16 top16 = (_Float16)w;
-            wf[0][i >> 3][i & 7] = top16;
-            wf[1][i >> 3][i & 7] = (_Float16)(w - (float)top16);
+            _Float16 hi, lo;
+            two_halves(e * up, hi, lo);
+            wf[0][i >> 3][i & 7] = hi, wf[1][i >> 3][i & 7] = lo;
         }
+        sum = or_not(sum, scores);
     }
     l = l * alpha + sum;
 }
@@ -544,8 +550,9 @@ __global__ __launch_bounds__(256) void attn_pages_merge_kernel(pcb_attn_pages_ar
         if (4 * q + 64 * k < dim) store4(op + 4 * q + 64 * k, v[k][0] * f, v[k][1] * f, v[k][2] * f, v[k][3] * f);
 }
 
-// How a call is cut.  Up to 32 columns a tile: in blocks of 16 or 32, the steps of everything shared out; more: blocks of 128, in key runs where these are too few to fill
-// the chip.
+// How a call is cut.  Up to 32 columns a tile (single tokens: any number): in blocks of 16 or 32, the steps of everything shared out to at most two workgroups a CU, one for every
+// four steps (three and four a CU: 64 single tokens 54 -> 60 .. 82 us); from 513 tiles on a workgroup a unit.  More columns: blocks of 128, in key runs where these are too few to
+// fill the chip twice.  A run has at least 16 steps, 8 where the units are less than half the chip's workgroups (always 8: 5 prompts of up to 700 rows, fp32, 36 -> 39 us).
 Plan plan_of(int64_t n_rows, int64_t H, int Hkv, int dim, int n_tiles, int tile_rows, int64_t longest) {
     Plan p{};
     p.per = (int)(H / Hkv);
@@ -569,8 +576,8 @@ Plan plan_of(int64_t n_rows, int64_t H, int Hkv, int dim, int n_tiles, int tile_
     }
     return p;
 }
-// Whether a unit's results are merged by the last of its workgroups: while these are few, a second launch costs more (us, two launches / one; 1 to 512 units of 4 columns and 1 to 64
-// results 17.6 / 15.0 to 194 / 190, 16 columns of 5 results 18.1 / 15.8, but of 32 16.9 / 18.3)
+// Whether a unit's results are merged by the last of its workgroups: while columns times results stay below 256 a second launch costs more (us, two launches / one; 1 to 512 units of
+// 4 columns and 1 to 63 results 17.6 / 15.0 to 194 / 190, 16 columns of 5 results 18.1 / 15.8, but of 32 16.9 / 18.3)
 bool merged_in_launch(const Plan& p, int Hkv, int n_tiles, int tile_rows) {
     const int64_t cols = (int64_t)tile_rows * p.per, units = (int64_t)n_tiles * Hkv * p.cblocks;
     return (cols < p.cols ? cols : p.cols) * (p.groups / units + 1) < 256;
