@@ -19,6 +19,7 @@ struct Plan {
     int cols, cblocks;                 // columns of a block, and the blocks of a full tile
     int groups;                        // few columns: workgroups that the steps are shared out to; 0: a workgroup takes all keys of its unit
     int runs, run;                     // many columns (cols = 128): key runs of a unit and their steps
+    int halves;                        // .. and whether a workgroup is eight waves, two for each of its columns
 };
 // what `part` holds.  Few columns: the sums of the tiles' costs (int32 [n_tiles + 1]) and a workgroup's share, then for two results of each workgroup [cols][dim] and [cols][2];
 // many columns: [dim] of each run of each (flat row, head), then all their pairs

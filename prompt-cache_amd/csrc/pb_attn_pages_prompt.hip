@@ -28,14 +28,17 @@ __device__ __forceinline__ float sum2(float v) {
 }
 __device__ __forceinline__ float lane_of(float v, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)); }
 
-// ND: value columns (and key elements) in blocks of 32
-template <typename E, int CODE, int ND>
-__global__ __launch_bounds__(256, sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_pages_prompt_kernel(pcb_attn_pages_args a, Plan pl) {
+// ND: value columns (and key elements) in blocks of 32.  KS = 2: eight waves, of which the second four take every other step with images of their own, so that a CU that has one
+// workgroup still has two waves a SIMD, one multiplying while the other one is at its softmax; their results meet in LDS.
+template <typename E, int CODE, int ND, int KS>
+__global__ __launch_bounds__(256 * KS, KS == 1 && sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_pages_prompt_kernel(pcb_attn_pages_args a, Plan pl) {
     constexpr bool F32 = sizeof(E) == 4;
     constexpr int PARTS = F32 ? 2 : 1, KK = 2 * ND;                   // k-steps of 16 of the first product
     constexpr int KLD = 32 * ND + 8, VLD = 72, PIECES = 128 * ND, NP = (PIECES + 255) / 256;   // sixteen-byte pieces of a step's keys, and of its values; of each a thread's
-    __shared__ __attribute__((aligned(16))) _Float16 Ks[2][64 * KLD], Vs[2][32 * ND * VLD];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, c = lane & 31;
+    constexpr int OLD = 32 * ND + 4;                                  // a column's sums, where the two halves of the waves meet
+    __shared__ __attribute__((aligned(16))) _Float16 images[KS][2][64 * KLD + 32 * ND * VLD];
+    const int tid = threadIdx.x & 255, kg = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, c = lane & 31;
     const int hk = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, cb = rest % pl.cblocks, t = a.n_tiles - 1 - rest / pl.cblocks;   // (a prompt's last tiles, which see most keys, first)
     const int dim = a.dim, ps = pl.ps, P = 1 << ps, per = pl.per;
     Tile tl = tile_of(a, t, ps);
@@ -58,8 +61,8 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_p
     int pages = -1;
     float kss = 1.0f, vss = 1.0f;
     auto look = [&](int s) {
-        const int key = (s + (lane >> 2)) * 64 + 16 * (lane & 3);
-        pages = s + (lane >> 2) < s1 && key < kv ? table[key >> ps] : -1;
+        const int key = (s + (lane >> 2) * KS) * 64 + 16 * (lane & 3);
+        pages = s + (lane >> 2) * KS < s1 && key < kv ? table[key >> ps] : -1;
         pages = pages >= 0 && pages < a.n_pages ? pages : -1;
         const int64_t ph = (int64_t)(pages < 0 ? 0 : pages) * a.Hkv + hk;
         kss = pages < 0 ? 1.0f : a.kscale[ph], vss = pages < 0 ? 1.0f : a.vscale[ph];
@@ -92,22 +95,23 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_p
         }
     };
     auto stage = [&](int buf) {
+        _Float16 *Ks = images[kg][buf], *Vs = Ks + 64 * KLD;
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             if (PIECES % 256 && n * 256 + tid >= PIECES) break;
             const int row = (n * 256 + tid) / (2 * ND), ch = (n * 256 + tid) % (2 * ND);
-            _Float16* k = &Ks[buf][row * KLD + 16 * ch];
+            _Float16* k = Ks + row * KLD + 16 * ch;
             *reinterpret_cast<h8*>(k) = half8<CODE>(u32x2{kr[n][0], kr[n][1]});
             *reinterpret_cast<h8*>(k + 8) = half8<CODE>(u32x2{kr[n][2], kr[n][3]});
-            _Float16* v = &Vs[buf][(n * 64 + (tid >> 2)) * VLD + 16 * vq];
+            _Float16* v = Vs + (n * 64 + (tid >> 2)) * VLD + 16 * vq;
             *reinterpret_cast<h8*>(v) = half8<CODE>(u32x2{vr[n][0], vr[n][1]});
             *reinterpret_cast<h8*>(v + 8) = half8<CODE>(u32x2{vr[n][2], vr[n][3]});
         }
     };
     int i = 0;
-    if (s0 < s1) {
-        look(s0);
-        fetch(s0, 0);
+    if (s0 + kg < s1) {
+        look(s0 + kg);
+        fetch(s0 + kg, 0);
     }
     // this lane's column
     const int col = col0 + 32 * wave + c;
@@ -158,10 +162,10 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_p
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
-    if (s0 < s1) stage(0);
+    if (s0 + kg < s1) stage(0);
     const int krow = (c >> 4) * 16 + ((c >> 2) & 1) * 8 + ((c >> 3) & 1) * 4 + (c & 3);   // the key of 32 that row c of the first product's operand is
     int buf = 0;
-    for (int s = s0; s < s1; ++s) {
+    for (int s = s0 + kg; s - kg < s1; s += KS) {
         // the step's scales, before `look` takes the next ones' place
         float ks[4], vs[4];
         bool whole = s * 64 + 64 <= all_hi && s * 64 >= all_lo;
@@ -172,20 +176,20 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_p
             page_ok |= (__builtin_amdgcn_readlane(pages, 4 * i + q) >= 0 ? 1 : 0) << q;
         }
         whole = whole && page_ok == 15;
-        const bool more = s + 1 < s1;
+        const bool more = s + KS < s1;
         __syncthreads();                                              // the step's image is written, the other one read
         i = (i + 1) & 15;
         if (more) {
-            if (i == 0) look(s + 1);
-            fetch(s + 1, i);
+            if (i == 0) look(s + KS);
+            fetch(s + KS, i);
         }
-        if (s * 64 < any_hi && s * 64 + 64 > any_lo) {
+        if ((KS == 1 || s < s1) && s * 64 < any_hi && s * 64 + 64 > any_lo) {
             f16v acc[2];
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[b][e] = 0.0f;
-                const _Float16* k = &Ks[buf][(32 * b + krow) * KLD + 8 * hh];
+                const _Float16* k = &images[kg][buf][(32 * b + krow) * KLD + 8 * hh];
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) {
                     const h8 f = *reinterpret_cast<const h8*>(k + 16 * kk);
@@ -255,7 +259,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_p
             for (int m = 0; m < 4; ++m) {
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    const h8 x = *reinterpret_cast<const h8*>(&Vs[buf][(32 * d + c) * VLD + 8 * hh + 16 * m]);
+                    const h8 x = *reinterpret_cast<const h8*>(&images[kg][buf][64 * KLD + (32 * d + c) * VLD + 8 * hh + 16 * m]);
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wf[p][m], o[d], 0, 0, 0);
                 }
@@ -264,8 +268,28 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_p
         if (more) stage(buf ^ 1);
         buf ^= 1;
     }
-    if (!live) return;
     l = sum2(l);
+    if constexpr (KS == 2) {
+        float* sums = reinterpret_cast<float*>(&images[0][0][0]) + (32 * wave + c) * (OLD + 2);
+        static_assert(128 * (OLD + 2) * 4 <= (int)sizeof(images), "the sums of 128 columns in the images' place");
+        __syncthreads();                                              // (all images have been multiplied)
+        if (kg == 1) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sums[32 * d + 8 * (e >> 2) + 4 * hh + (e & 3)] = o[d][e];
+            if (hh == 0) sums[OLD] = M, sums[OLD + 1] = l;
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const float M1 = sums[OLD], top = fmaxf(M, M1), use = top == NEG ? 0.0f : top, x = pow_of<E>(M - use), y = pow_of<E>(M1 - use);
+        M = top, l = l * x + sums[OLD + 1] * y;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] = o[d][e] * x + sums[32 * d + 8 * (e >> 2) + 4 * hh + (e & 3)] * y;
+    }
+    if (!live) return;
     E* op = (E*)a.out + ((int64_t)tl.row0 + qr) * a.ldo + (int64_t)h * a.out_head_stride;
     const int64_t at_part = (((int64_t)tl.row0 + qr) * a.H + h) * pl.runs + blockIdx.y;
     float* pp = a.part + at_part * dim;
@@ -284,20 +308,30 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_p
         }
 }
 
+template <typename E, int CODE, int ND, int KS>
+void launch_one(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
+    const dim3 grid((unsigned)((int64_t)a.n_tiles * a.Hkv * pl.cblocks), pl.runs);
+    hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, ND, KS>), grid, dim3(256 * KS), 0, stream, a, pl);
+}
 template <typename E, int CODE>
 int launch(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
-    const dim3 grid((unsigned)((int64_t)a.n_tiles * a.Hkv * pl.cblocks), pl.runs), block(256);
     const int blocks = (a.dim + 31) / 32;
-    if (blocks <= 2)
-        hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 2>), grid, block, 0, stream, a, pl);
+    if (pl.halves && blocks <= 2)
+        launch_one<E, CODE, 2, 2>(a, pl, stream);
+    else if (pl.halves && blocks == 3)
+        launch_one<E, CODE, 3, 2>(a, pl, stream);
+    else if (pl.halves && blocks == 4)
+        launch_one<E, CODE, 4, 2>(a, pl, stream);
+    else if (blocks <= 2)
+        launch_one<E, CODE, 2, 1>(a, pl, stream);
     else if (blocks == 3)
-        hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 3>), grid, block, 0, stream, a, pl);
+        launch_one<E, CODE, 3, 1>(a, pl, stream);
     else if (blocks == 4)
-        hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 4>), grid, block, 0, stream, a, pl);
+        launch_one<E, CODE, 4, 1>(a, pl, stream);
     else if (blocks <= 6)
-        hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 6>), grid, block, 0, stream, a, pl);
+        launch_one<E, CODE, 6, 1>(a, pl, stream);
     else
-        hipLaunchKernelGGL((attn_pages_prompt_kernel<E, CODE, 8>), grid, block, 0, stream, a, pl);
+        launch_one<E, CODE, 8, 1>(a, pl, stream);
     return pcb_check_launch("attn_pages_prompt_kernel");
 }
 

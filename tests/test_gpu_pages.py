@@ -507,6 +507,16 @@ def test_attention_in_a_graph_is_the_eager_one_but_for_its_merge():
         r.check(out)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dim, kind", [(48, "e4m3"), (80, "int8"), (128, "e4m3")])
+def test_attention_of_more_blocks_than_the_chip_has_cus(dim, kind, dtype):
+    rng = np.random.default_rng(dim)
+    n = 70
+    r = Requests([int(v) for v in rng.integers(0, 300, n)], [int(v) for v in rng.integers(30, 41, n)], 8, 4, dim, 32, kind, dtype, seed=dim)
+    r.check(r.run(40))
+    r.check(r.run(40, window=50), window=50)
+
+
 def test_attention_of_more_tiles_than_are_shared_out():
     """Over 512 tiles: a workgroup a unit."""
     n = 600
