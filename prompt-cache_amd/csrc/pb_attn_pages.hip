@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
     _Float16* const Qs = reinterpret_cast<_Float16*>(&Os[0][0][0]);  // (before there are results)
     __shared__ float Ms[NW][COLS], Ls[NW][COLS];
     __shared__ __attribute__((aligned(16))) int4 tiles_s[SHARED_TILES];
-    __shared__ int starts[SHARED_TILES + 1], kv_s[SHARED_TILES], wsum[NW], found_s, last_s;
+    __shared__ int starts[SHARED_TILES + 1], kv_s[SHARED_TILES], wsum[NW], last_s;
     __shared__ float unit_s[COLS];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int per = pl.per, dim = a.dim, ps = pl.ps, P = 1 << ps;
@@ -154,19 +154,20 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
     if (pl.groups) {
         const int tid = threadIdx.x, lane = tid & 63;
         int all = 0;
-        for (int t0 = 0; t0 < a.n_tiles; t0 += NT) {
-            int n = 0;
-            if (t0 + tid < a.n_tiles) {
-                const Tile x = tile_of(a, t0 + tid, ps);
-                tiles_s[t0 + tid] = int4{x.seq, x.pos, x.rows, x.row0}, kv_s[t0 + tid] = x.kv;
-                n = (max(x.s1 - x.s0, 1) + UNIT_STEPS) * a.Hkv * ((x.rows * per + COLS - 1) / COLS);
-            }
-            int v = n;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int u = __shfl_up(v, o, 64);
-                if (lane >= o) v += u;
-            }
+        auto cost_of = [&](int t) {
+            if (t >= a.n_tiles) return 0;
+            const Tile x = tile_of(a, t, ps);
+            tiles_s[t] = int4{x.seq, x.pos, x.rows, x.row0}, kv_s[t] = x.kv;
+            return (max(x.s1 - x.s0, 1) + UNIT_STEPS) * a.Hkv * ((x.rows * per + COLS - 1) / COLS);
+        };
+        if (a.n_tiles <= 64) {                                        // (every wave for itself: the same numbers)
+            const int n = cost_of(lane), v = wave_scan(n);
+            if (lane < a.n_tiles) starts[lane] = v - n;
+            all = __builtin_amdgcn_readlane(v, 63);
+        }
+        for (int t0 = 0; a.n_tiles > 64 && t0 < a.n_tiles; t0 += NT) {
+            const int n = cost_of(t0 + tid);
+            int v = wave_scan(n);
             if (lane == 63) wsum[wave] = v;
             __syncthreads();
             int sum = 0;
@@ -194,23 +195,27 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
     const int at0 = at;
     float* const part = a.part + head_floats(a.n_tiles);
     while (at < end) {
-        int t, j, from, steps, n_steps, mine = 1, g0 = 0, parts = 1, second = 0;  // unit j of tile t, its steps from .. from + n_steps - 1; the workgroups that share it are g0 ..
+        int t, j, from, steps, n_steps, mine = 1, u0 = 0;    // unit j of tile t, whose place among all is u0; its steps from .. from + n_steps - 1
         Tile tl;
         if (pl.groups) {
-            for (int i = threadIdx.x; i < a.n_tiles; i += NT)
-                if (starts[i] <= at && at < starts[i + 1]) found_s = i;
-            __syncthreads();
-            t = __builtin_amdgcn_readfirstlane(found_s);
+            t = 0;
+            for (int i = threadIdx.x & 63; t < a.n_tiles; i += 64, t += 64) {   // (every wave by itself; `at` is in one)
+                const uint64_t here = __ballot(i < a.n_tiles && starts[i] <= at && at < starts[i + 1]);
+                if (here) {
+                    t += __builtin_ctzll(here);
+                    break;
+                }
+            }
             const int4 rec = tiles_s[t];
             tl.seq = __builtin_amdgcn_readfirstlane(rec.x), tl.pos = __builtin_amdgcn_readfirstlane(rec.y), tl.rows = __builtin_amdgcn_readfirstlane(rec.z);
             tl.row0 = __builtin_amdgcn_readfirstlane(rec.w), tl.kv = __builtin_amdgcn_readfirstlane(kv_s[t]);
             tl = rows_of(a, tl, 0, tl.rows - 1);
             steps = max(tl.s1 - tl.s0, 1);
             const int off = at - __builtin_amdgcn_readfirstlane(starts[t]), cost = steps + UNIT_STEPS;
-            j = off / cost;
+            j = (int)((uint32_t)off / (uint32_t)cost);
             const int p = off - j * cost;
             mine = min(cost - p, end - at);
-            g0 = (at - p + UNIT_STEPS) / share, parts = (at - p + cost - 1) / share - g0 + 1, second = at - p > g0 * share;
+            u0 = at - p;
             from = max(p - UNIT_STEPS, 0), n_steps = max(p + mine - UNIT_STEPS, 0) - from;
         } else {
             t = blockIdx.x, j = blockIdx.y;
@@ -423,6 +428,8 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // (every wave's results have left it before one of them answers for all)
         __syncthreads();
         if (unit || !a.counters) continue;
+        // the workgroups that share the unit: g0 .. g0 + parts - 1, the first one's result its second where it had another unit's before
+        const int g0 = (int)((uint32_t)(u0 + UNIT_STEPS) / (uint32_t)share), parts = (int)((uint32_t)(u0 + steps + UNIT_STEPS - 1) / (uint32_t)share) - g0 + 1, second = u0 > g0 * share;
         // The last of the unit's workgroups merges: its fellows' results were past the caches before they were counted.
         if (tid == 0) {
             last_s = __hip_atomic_fetch_add(&a.counters[g0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;

@@ -17,6 +17,23 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float fp2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
+// inclusive sums over a wave of which all lanes are active: within rows of sixteen, then their last lanes' over the next rows (no LDS, 6 steps)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t moved(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)moved<CTRL, ROWS>((int)v) | (uint64_t)(uint32_t)moved<CTRL, ROWS>((int)(v >> 32)) << 32);
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v += moved<0x111, 0xf>(v);                                        // row_shr 1, 2, 4, 8
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);                                        // row_bcast 15, 31
+    return v + moved<0x143, 0xc>(v);
+}
+
 constexpr int SCALE_EXP = 40;      // exponents of scales: -40 .. 40.  The softmax weights times two scales' quotient then stay far inside fp32
 
 template <int CODE>

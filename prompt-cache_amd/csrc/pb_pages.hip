@@ -14,31 +14,25 @@ namespace {
 using namespace pcb;
 
 // ---- tables -------------------------------------------------------------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ T wave_scan(T v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const T u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
-    return v;
-}
-// inclusive sums over the workgroup's threads; `all`: the whole sum
-template <int NT, typename T>
-__device__ __forceinline__ T block_scan(T v, T* part, int tid, T& all) {
+// K inclusive sums over the workgroup's threads; `all`: the whole sums.  One barrier: `part` belongs to one call of a chunk
+template <int NT, int K, typename T>
+__device__ __forceinline__ void block_scan(T (&v)[K], T (*part)[NT / 64], int tid, T (&all)[K]) {
     const int lane = tid & 63, wave = tid >> 6;
-    v = wave_scan(v, lane);
-    __syncthreads();
-    if (lane == 63) part[wave] = v;
-    __syncthreads();
-    T before = 0;
-    all = 0;
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) {
-        if (w < wave) before += part[w];
-        all += part[w];
+    for (int k = 0; k < K; ++k) {
+        v[k] = wave_scan(v[k]);
+        if (lane == 63) part[k][wave] = v[k];
     }
-    return before + v;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        all[k] = 0;
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) {
+            if (w == wave) v[k] += all[k];
+            all[k] += part[k][w];
+        }
+    }
 }
 // the first thread whose sum is above x
 template <int NT>
@@ -57,8 +51,8 @@ __device__ __forceinline__ int ring_at(int64_t i, int cap) { return (int)(i % ca
 
 template <int NT>
 __global__ __launch_bounds__(NT) void page_tables_kernel(pcb_page_tables_args a, int ps) {
-    __shared__ int64_t part64[NT / 64];
-    __shared__ int part[NT / 64];
+    __shared__ int64_t part64[1][NT / 64];
+    __shared__ int part_need[1][NT / 64], part[5][NT / 64];
     __shared__ int stop_s[NT], take_s[NT], back_s[NT], tile_s[NT];    // inclusive sums over the chunk: rows, pages taken, pages given back, tiles
     __shared__ int cached_s[NT], have_s[NT], keep_s[NT], count_s[NT]; // count: rows of a granted sequence, -1 where not granted
     __shared__ int last;
@@ -78,21 +72,23 @@ __global__ __launch_bounds__(NT) void page_tables_kernel(pcb_page_tables_args a,
         const int count = over ? 0 : brings;
         const int have = (int)(((int64_t)cached + P - 1) >> ps);
         const int64_t total = ((int64_t)cached + count + P - 1) >> ps;
-        int64_t rows_all;
-        const int64_t stop = rows0 + block_scan<NT>((int64_t)count, part64, tid, rows_all);
+        int64_t rows_sum[1] = {(int64_t)count}, rows_whole[1];
+        block_scan<NT>(rows_sum, part64, tid, rows_whole);
+        const int64_t rows_all = rows_whole[0], stop = rows0 + rows_sum[0];
         const bool fits = total <= a.max_pages && stop <= a.n_rows;
         const int need = a.ring && live && !over && fits ? (int)total - have : 0;
-        int need_all;
-        const int upto = need0 + block_scan<NT>(need, part, tid, need_all);
-        const bool granted = live && !over && fits && (need == 0 || upto <= free_pages);
+        int need_sum[1] = {need}, need_all[1];
+        block_scan<NT>(need_sum, part_need, tid, need_all);
+        const bool granted = live && !over && fits && (need == 0 || need0 + need_sum[0] <= free_pages);
         int keep = over && a.keep ? a.keep[s] : 0;
         keep = keep < 0 ? 0 : keep;
         const int back = a.ring && over && have <= a.max_pages && have > keep ? have - keep : 0;
         const int tiles = granted ? (int)(((int64_t)count + a.tile_rows - 1) / a.tile_rows) : 0;
-        int take_all, back_all, tile_all;
-        take_s[tid] = block_scan<NT>(granted ? need : 0, part, tid, take_all);
-        back_s[tid] = block_scan<NT>(back, part, tid, back_all);
-        tile_s[tid] = block_scan<NT>(tiles, part, tid, tile_all);
+        int sums[5] = {granted ? need : 0, back, tiles, live && !over && !granted ? 1 : 0, granted ? count : 0}, whole[5];
+        block_scan<NT>(sums, part, tid, whole);
+        const int take_all = whole[0], back_all = whole[1], tile_all = whole[2];
+        take_s[tid] = sums[0], back_s[tid] = sums[1], tile_s[tid] = sums[2];
+        refused += whole[3], given += whole[4];
         stop_s[tid] = (int)(stop - rows0 > a.n_rows ? (int64_t)a.n_rows + 1 : stop - rows0);   // (rows behind n_rows are nobody's)
         cached_s[tid] = cached, have_s[tid] = have, keep_s[tid] = keep, count_s[tid] = granted ? count : -1;
         if (wg == 0) {
@@ -103,13 +99,6 @@ __global__ __launch_bounds__(NT) void page_tables_kernel(pcb_page_tables_args a,
                     a.row_start[s] = (int)(first > 0x7fffffff ? 0x7fffffff : first);
                     if (s == a.n_seqs - 1) a.row_start[a.n_seqs] = (int)(stop > 0x7fffffff ? 0x7fffffff : stop);
                 }
-            }
-            if (a.status) {
-                int n;
-                block_scan<NT>(live && !over && !granted ? 1 : 0, part, tid, n);
-                refused += n;
-                block_scan<NT>(granted ? count : 0, part, tid, n);
-                given += n;
             }
         }
         __syncthreads();
@@ -150,7 +139,7 @@ __global__ __launch_bounds__(NT) void page_tables_kernel(pcb_page_tables_args a,
                 rec.w = (int)(rows0 + (t ? stop_s[t - 1] : 0)) + off;
                 if (tile0 + i < a.n_tiles) reinterpret_cast<int4*>(a.tiles)[tile0 + i] = rec;
             }
-        rows0 += rows_all, need0 += need_all, take0 += take_all, back0 += back_all, tile0 += tile_all;
+        rows0 += rows_all, need0 += need_all[0], take0 += take_all, back0 += back_all, tile0 += tile_all;
         __syncthreads();
     }
     for (int64_t r = rows0 + wg * NT + tid; r < a.n_rows; r += gsz * NT) {
