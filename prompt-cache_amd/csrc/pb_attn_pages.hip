@@ -557,11 +557,13 @@ __global__ __launch_bounds__(256) void attn_pages_merge_kernel(pcb_attn_pages_ar
         if (4 * q + 64 * k < dim) store4(op + 4 * q + 64 * k, v[k][0] * f, v[k][1] * f, v[k][2] * f, v[k][3] * f);
 }
 
-// How a call is cut.  Up to 32 columns a tile (single tokens: any number): in blocks of 16 or 32, the steps of everything shared out to at most two workgroups a CU, one for every
-// four steps (three and four a CU: 64 single tokens 54 -> 60 .. 82 us); from 513 tiles on a workgroup a unit.  More columns: blocks of 128, in key runs where these are too few to
-// fill the chip twice, of at least 16 steps, 8 where the blocks are less than 128 (always 8: 5 prompts of up to 600 rows, fp32, 29.0 -> 33.8 us).  Where that comes to a workgroup a CU at
-// most, heads up to 128, it has eight waves (us, without / with): 216 blocks of 12 heads of 96 27.6 / 21.4, in fp32 39.0 / 32.0; few blocks are then cut for one a CU, not
-// two: 64 rows of 32 heads of 64 over 16 000 keys 31.6 / 25.9, 512 of 16 of 128 over 2 000 37.5 / 31.8 (but 1 500 of 8 heads on their own, fp32, 38.4 / 42.7: the last rows' blocks see all keys).
+// How a call is cut.  Up to 32 columns a tile (single tokens: any number): in blocks of 16 or 32, the steps of everything shared out to at most two workgroups a CU (three and four:
+// 64 single tokens 54 -> 60 .. 82 us), one for every eight steps (16 over 1 000 keys 15.9 us, for every four 18.6) or four of 32 columns (20 rows over 4 000 22.4, eight 23.9); from
+// 513 tiles on a workgroup a unit.
+// More columns: blocks of 128, in key runs where these are too few to fill the chip twice, of at least 16 steps, 8 where the blocks are less than 128 (always 8: 5 prompts of up to 600
+// rows, fp32, 29.0 -> 33.8 us).  Where that comes to a workgroup a CU at most, heads up to 128, it has eight waves (us, without / with): 216 blocks of 12 heads of 96 27.6 / 21.4, in
+// fp32 39.0 / 32.0; few blocks are then cut for one a CU, not two: 64 rows of 32 heads of 64 over 16 000 keys 31.6 / 25.9, 512 of 16 of 128 over 2 000 37.5 / 31.8 (but 1 500 of 8
+// heads on their own, fp32, 38.4 / 42.7: the last rows' blocks see all keys).
 Plan plan_of(int64_t n_rows, int64_t H, int Hkv, int dim, int n_tiles, int tile_rows, int64_t longest) {
     Plan p{};
     p.per = (int)(H / Hkv);
@@ -582,8 +584,9 @@ Plan plan_of(int64_t n_rows, int64_t H, int Hkv, int dim, int n_tiles, int tile_
         // (a workgroup a CU at most: eight waves each)
         p.halves = dim <= 128 && units * p.runs <= 256 && steps > 1 && (int64_t)n_tiles * Hkv * p.cblocks < 1 << 22;
     } else if (n_tiles <= SHARED_TILES && steps > 8) {
-        const int64_t fours = (units * steps + 3) / 4;
-        p.groups = (int)(fours < MAX_GROUPS ? fours : MAX_GROUPS);
+        const int each = p.cols == 32 ? 4 : 8;
+        const int64_t n = (units * steps + each - 1) / each;
+        p.groups = (int)(n < MAX_GROUPS ? n : MAX_GROUPS);
     }
     return p;
 }

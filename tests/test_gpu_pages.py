@@ -437,11 +437,11 @@ def test_attention_passes_over_tiles_that_are_none(T):
     r = Requests([700, 40], [33, 2], 4, 2, 64, 32, "e4m3", "bf16", seed=9)
     top = 2 ** 31 - 1
     none = [[-1, 0, 1, 0], [2, 0, 1, 0], [0, -1, 1, 0], [0, 5, 0, 0], [0, 5, -3, 0], [0, 5, 1, 35], [0, 5, 1, -1], [0, 5, 1, top], [top, top, top, top], [0, top, 1, 0], [1, top - T + 1, T, 0]]
-    want = r.run(T)
     for window in (0, 30):
         got = r.run(T, window=window, tiles=none)
         assert bool((got == 55).all())
-    assert torch.equal(want, r.run(T, tiles=none[:5] + r.tiles(T) + none[5:]))
+        # (more tiles are cut into other key runs: other orders of the same sums)
+        r.check(r.run(T, window=window, tiles=none[:5] + r.tiles(T) + none[5:]), window=window)
 
 
 @pytest.mark.parametrize("T", [1, 9, 64])
