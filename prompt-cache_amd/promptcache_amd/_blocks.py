@@ -5,6 +5,7 @@ and a failing call raises ``RuntimeError`` with the library's own message.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
 
 import torch
@@ -291,11 +292,11 @@ SIGNATURES = {
     "pcb_rec_prompt": (C.c_int, [C.POINTER(RecArgs), _vp]),
     "pcb_rec_step_fits": (C.c_int32, [_i32, _i32]),
     "pcb_rec_step": (C.c_int, [C.POINTER(RecArgs), _vp]),
-    "pcb_page_tables": (C.c_int, [C.POINTER(PageTablesArgs), _vp]),
-    "pcb_pages_append": (C.c_int, [C.POINTER(PagesRowsArgs), _vp]),
-    "pcb_pages_read": (C.c_int, [C.POINTER(PagesRowsArgs), _vp]),
+    "pcb_page_tables": (C.c_int, [_vp, _vp]),
+    "pcb_pages_append": (C.c_int, [_vp, _vp]),
+    "pcb_pages_read": (C.c_int, [_vp, _vp]),
     "pcb_attn_pages_part": (_i64, [_i32] * 7),
-    "pcb_attn_pages": (C.c_int, [C.POINTER(AttnPagesArgs), _vp]),
+    "pcb_attn_pages": (C.c_int, [_vp, _vp]),
 }
 
 
@@ -1190,10 +1191,19 @@ _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _flat(t: Optional[torch.Tensor], dtype, numel: int, dev: int, what: str) -> Optional[int]:
-    """The address of ``t`` (optional), which holds at least ``numel`` elements of ``dtype`` one after the other on device ``dev``."""
+def _packed(cls):
+    """What lays out a struct's fields as ``cls`` does, its size in front: (fields behind ``struct_bytes``) -> bytes.  (A third of what making the struct itself takes.)"""
+    kinds = {C.c_uint32: "I", _i32: "i", _i64: "q", _f32: "f", _vp: "P"}
+    s = struct.Struct("@" + "".join(kinds[t] for _, t in cls._fields_) + "0q")
+    size = C.sizeof(cls)
+    assert s.size == size
+    return lambda *fields: s.pack(size, *fields)
+
+
+def _flat(t: Optional[torch.Tensor], dtype, numel: int, dev: int, what: str) -> int:
+    """The address of ``t`` (None: 0), which holds at least ``numel`` elements of ``dtype`` one after the other on device ``dev``."""
     if t is None:
-        return None
+        return 0
     if t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and t.numel() >= numel:
         return t.data_ptr()
     if t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
@@ -1246,7 +1256,7 @@ def _table(table: torch.Tensor, n: int, dev: int, what: str):
     return table.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], shape[1]), shape[1]
 
 
-_TABLES_BYTES, _ROWS_BYTES, _ATTN_BYTES = C.sizeof(PageTablesArgs), C.sizeof(PagesRowsArgs), C.sizeof(AttnPagesArgs)
+_tables_args, _rows_args, _attn_args = _packed(PageTablesArgs), _packed(PagesRowsArgs), _packed(AttnPagesArgs)
 
 
 def page_tables(cached: torch.Tensor, brings: torch.Tensor, table: torch.Tensor, page_size: int, *, row_slot: torch.Tensor, kv_len=None, row_start=None, row_seq=None,
@@ -1258,11 +1268,11 @@ def page_tables(cached: torch.Tensor, brings: torch.Tensor, table: torch.Tensor,
     n, rows = cached.numel(), row_slot.numel()
     dev = _device_of(cached, "page_tables cached")
     tab, ld, pages = _table(table, n, dev, "page_tables")
-    a = PageTablesArgs(_TABLES_BYTES, n, pages, ld, page_size, _flat(cached, _I32, n, dev, "cached"), _flat(brings, _I32, n, dev, "brings"), _flat(keep, _I32, n, dev, "keep"),
-                       tab, _flat(ring, _I32, 1, dev, "ring"), 0 if ring is None else ring.numel(), _flat(ring_state, _I32, 2, dev, "ring_state"),
-                       _flat(ring_out, _I32, 4, dev, "ring_out"), _flat(kv_len, _I32, n, dev, "kv_len"), _flat(row_start, _I32, n + 1, dev, "row_start"),
-                       _flat(row_seq, _I32, rows, dev, "row_seq"), _flat(row_pos, _I32, rows, dev, "row_pos"), _flat(row_slot, _I64, rows, dev, "row_slot"), rows,
-                       _flat(tiles, _I32, 0, dev, "tiles"), 0 if tiles is None else tiles.numel() // 4, tile_rows, _flat(status, _I32, 2, dev, "status"))
+    a = _tables_args(n, pages, ld, page_size, _flat(cached, _I32, n, dev, "cached"), _flat(brings, _I32, n, dev, "brings"), _flat(keep, _I32, n, dev, "keep"),
+                     tab, _flat(ring, _I32, 1, dev, "ring"), 0 if ring is None else ring.numel(), _flat(ring_state, _I32, 2, dev, "ring_state"),
+                     _flat(ring_out, _I32, 4, dev, "ring_out"), _flat(kv_len, _I32, n, dev, "kv_len"), _flat(row_start, _I32, n + 1, dev, "row_start"),
+                     _flat(row_seq, _I32, rows, dev, "row_seq"), _flat(row_pos, _I32, rows, dev, "row_pos"), _flat(row_slot, _I64, rows, dev, "row_slot"), rows,
+                     _flat(tiles, _I32, 0, dev, "tiles"), 0 if tiles is None else tiles.numel() // 4, tile_rows, _flat(status, _I32, 2, dev, "status"))
     rc = (_lib or load()).pcb_page_tables(a, _raw_stream(dev))
     if rc:
         check(rc, "pcb_page_tables")
@@ -1277,8 +1287,8 @@ def _pages_rows(name: str, k, v, row_slot, kcodes, kscale, vcodes, vscale) -> No
     if k.dtype is not v.dtype or shape != v.shape:
         raise TypeError(f"{name}: keys and values of one type and shape, got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
     rows = shape[0]
-    a = PagesRowsArgs(_ROWS_BYTES, _code(k), code, *_heads(k, Hkv, dim, dev, name), *_heads(v, Hkv, dim, dev, name), _flat(row_slot, _I64, rows, dev, "row_slot"), rows,
-                      kcodes.data_ptr(), kscale.data_ptr(), vcodes.data_ptr(), vscale.data_ptr(), pages, P, Hkv, dim)
+    a = _rows_args(_code(k), code, *_heads(k, Hkv, dim, dev, name), *_heads(v, Hkv, dim, dev, name), _flat(row_slot, _I64, rows, dev, "row_slot"), rows,
+                   kcodes.data_ptr(), kscale.data_ptr(), vcodes.data_ptr(), vscale.data_ptr(), pages, P, Hkv, dim)
     lib = _lib or load()
     rc = (lib.pcb_pages_append if name == "pages_append" else lib.pcb_pages_read)(a, _raw_stream(dev))
     if rc:
@@ -1340,10 +1350,10 @@ def attn_pages(q: torch.Tensor, tiles: torch.Tensor, tile_rows: int, kv_len: tor
     stream = _raw_stream(dev)
     if counters is None and part is not None:
         counters = _stream_counters(dev, stream, q.device)
-    a = AttnPagesArgs(_ATTN_BYTES, _code(q), code, *_heads(q, H, dim, dev, "attn_pages queries"), _flat(tiles, _I32, 0, dev, "attn_pages tiles"), n_tiles, tile_rows, rows,
-                      _flat(kv_len, _I32, 0, dev, "attn_pages kv_len"), tab, ld, n, wide, kcodes.data_ptr(), kscale.data_ptr(), vcodes.data_ptr(), vscale.data_ptr(), pages, P, H,
-                      Hkv, dim, scale, window, _flat(sink, _F32, H, dev, "attn_pages sink"), *_heads(out, H, dim, dev, "attn_pages results"), longest,
-                      _flat(part, _F32, 0, dev, "attn_pages part"), 0 if part is None else part.numel(), _flat(counters, _I32, 512, dev, "attn_pages counters"))
+    a = _attn_args(_code(q), code, *_heads(q, H, dim, dev, "attn_pages queries"), _flat(tiles, _I32, 0, dev, "attn_pages tiles"), n_tiles, tile_rows, rows,
+                   _flat(kv_len, _I32, 0, dev, "attn_pages kv_len"), tab, ld, n, wide, kcodes.data_ptr(), kscale.data_ptr(), vcodes.data_ptr(), vscale.data_ptr(), pages, P, H,
+                   Hkv, dim, scale, window, _flat(sink, _F32, H, dev, "attn_pages sink"), *_heads(out, H, dim, dev, "attn_pages results"), longest,
+                   _flat(part, _F32, 0, dev, "attn_pages part"), 0 if part is None else part.numel(), _flat(counters, _I32, 512, dev, "attn_pages counters"))
     rc = (_lib or load()).pcb_attn_pages(a, stream)
     if rc:
         check(rc, "pcb_attn_pages")
