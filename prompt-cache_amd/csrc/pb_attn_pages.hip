@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
         }
         all = __builtin_amdgcn_readfirstlane(all);
         share = (all + pl.groups - 1) / pl.groups;
-        share = share < NW + UNIT_STEPS ? NW + UNIT_STEPS : share;
+        share = share < MIN_SHARE ? MIN_SHARE : share;
         if (tid == 0) starts[a.n_tiles] = all;
         __syncthreads();
         if (blockIdx.x == 0 && !a.counters) {                         // for the launch that merges
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
             const int p = off - j * cost;
             mine = min(cost - p, end - at);
             u0 = at - p;
-            from = max(p - UNIT_STEPS, 0), n_steps = max(p + mine - UNIT_STEPS, 0) - from;
+            from = step_at(p, steps), n_steps = step_at(p + mine, steps) - from;
         } else {
             t = blockIdx.x, j = blockIdx.y;
             tl = tile_of(a, t, ps);
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
         const bool unit = n_steps == steps;
         const int slot = unit ? 0 : 2 * (int)blockIdx.x + (at == at0 ? 0 : 1);
         at += mine;
-        if (n_steps == 0) continue;                                   // (the share ends before the unit's first step)
+        if (n_steps == 0) continue;                                   // (the share ends in front of the unit's first steps, or begins behind its last ones)
         int tid = threadIdx.x;
         asm("" : "+v"(tid));                                          // (what hangs on it is computed anew for every unit: kept over the loop it takes the inner one's registers)
         const int lane = tid & 63, g = lane >> 4, c = lane & 15;
@@ -429,7 +429,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
         __syncthreads();
         if (unit || !a.counters) continue;
         // the workgroups that share the unit: g0 .. g0 + parts - 1, the first one's result its second where it had another unit's before
-        const int g0 = (int)((uint32_t)(u0 + UNIT_STEPS) / (uint32_t)share), parts = (int)((uint32_t)(u0 + steps + UNIT_STEPS - 1) / (uint32_t)share) - g0 + 1, second = u0 > g0 * share;
+        const int g0 = first_share(u0, steps, share), parts = last_share(u0, steps, share) - g0 + 1, second = u0 > g0 * share;
         // The last of the unit's workgroups merges: its fellows' results were past the caches before they were counted.
         if (tid == 0) {
             last_s = __hip_atomic_fetch_add(&a.counters[g0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
@@ -515,9 +515,9 @@ __global__ __launch_bounds__(256) void attn_pages_merge_kernel(pcb_attn_pages_ar
         const float* part = a.part + head_floats(a.n_tiles);
         const int64_t result = (int64_t)pl.cols * (dim + 2);
         const int share = head[a.n_tiles + 1];
-        const int steps = max(tl.s1 - tl.s0, 1), u0 = head[t] + (steps + UNIT_STEPS) * (cblock * a.Hkv + hk), s0 = u0 + UNIT_STEPS;   // the unit's and its first step's place among all
-        const int g0 = s0 / share;
-        n = (s0 + steps - 1) / share - g0 + 1;
+        const int steps = max(tl.s1 - tl.s0, 1), u0 = head[t] + (steps + UNIT_STEPS) * (cblock * a.Hkv + hk);   // the unit's place among all
+        const int g0 = first_share(u0, steps, share);
+        n = last_share(u0, steps, share) - g0 + 1;
         const float *first = part + (2 * (int64_t)g0 + (u0 > g0 * share ? 1 : 0)) * result, *second = part + 2 * ((int64_t)g0 + 1) * result;
         sum0 = first + cc * dim, max0 = first + pl.cols * dim + 2 * cc, sum1 = second + cc * dim, max1 = second + pl.cols * dim + 2 * cc, sum_step = max_step = 2 * result;
     }
