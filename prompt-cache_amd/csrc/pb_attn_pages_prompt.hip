@@ -31,12 +31,14 @@ __device__ __forceinline__ float lane_of(float v, int i) { return __uint_as_floa
 // ND: value columns (and key elements) in blocks of 32.  KS = 2: eight waves, of which the second four take every other step with images of their own, so that a CU that has one
 // workgroup still has two waves a SIMD, one multiplying while the other one is at its softmax; their results meet in LDS.
 template <typename E, int CODE, int ND, int KS>
-__global__ __launch_bounds__(256 * KS, KS == 1 && sizeof(E) == 2 && ND <= 4 ? 2 : 1) void attn_pages_prompt_kernel(pcb_attn_pages_args a, Plan pl) {
+__global__ __launch_bounds__(256 * KS, KS == 1 && sizeof(E) == 2 && ND <= 6 ? 2 : 1) void attn_pages_prompt_kernel(pcb_attn_pages_args a, Plan pl) {
     constexpr bool F32 = sizeof(E) == 4;
     constexpr int PARTS = F32 ? 2 : 1, KK = 2 * ND;                   // k-steps of 16 of the first product
     constexpr int KLD = 32 * ND + 8, VLD = 72, PIECES = 128 * ND, NP = (PIECES + 255) / 256;   // sixteen-byte pieces of a step's keys, and of its values; of each a thread's
     constexpr int OLD = 32 * ND + 4;                                  // a column's sums, where the two halves of the waves meet
-    __shared__ __attribute__((aligned(16))) _Float16 images[KS][2][64 * KLD + 32 * ND * VLD];
+    // (bf16 heads of 192: one image, and so two workgroups a CU: 2 000 rows of 32 heads over 4 000 keys 391 -> 305 us; 256 elements' sums and queries leave no registers for two)
+    constexpr int BUFS = !F32 && ND == 6 ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) _Float16 images[KS][BUFS][64 * KLD + 32 * ND * VLD];
     const int tid = threadIdx.x & 255, kg = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, c = lane & 31;
     const int hk = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, cb = rest % pl.cblocks, t = a.n_tiles - 1 - rest / pl.cblocks;   // (a prompt's last tiles, which see most keys, first)
@@ -265,8 +267,9 @@ __global__ __launch_bounds__(256 * KS, KS == 1 && sizeof(E) == 2 && ND <= 4 ? 2 
                 }
             }
         }
-        if (more) stage(buf ^ 1);
-        buf ^= 1;
+        if (BUFS == 1) __syncthreads();                               // (the image has been read)
+        if (more) stage(BUFS == 1 ? 0 : buf ^ 1);
+        if (BUFS == 2) buf ^= 1;
     }
     l = sum2(l);
     if constexpr (KS == 2) {
