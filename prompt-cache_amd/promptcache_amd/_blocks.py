@@ -1256,6 +1256,15 @@ def _table(table: torch.Tensor, n: int, dev: int, what: str):
     return table.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], shape[1]), shape[1]
 
 
+_looks = (_flat, _heads, _table, _pool)
+try:                                                               # (the same looks in a call each, where they were compiled for this torch: 2 to 4 us of a call's 9 to 12)
+    from . import _tensors
+    if _tensors.torch_version == torch.__version__.split("+")[0]:
+        _tensors.behind(*_looks)
+        _flat, _heads, _table, _pool = _tensors.flat, _tensors.heads, _tensors.table, _tensors.pool
+except ImportError:
+    pass
+
 _tables_args, _rows_args, _attn_args = _packed(PageTablesArgs), _packed(PagesRowsArgs), _packed(AttnPagesArgs)
 
 

@@ -2,7 +2,8 @@
 
 The package's kernels come in groups that build and load independently, so that a process pays only for what its model uses:
 ``pc_*.hip`` -> ``libpromptcache_hip.so`` (the split-precision fp16 stacks of the Llama / Falcon / MPT adapters) and
-``pb_*.hip`` -> ``libpromptcache_blocks.so`` (the bf16 / fp32 building blocks).  One hipcc per translation unit, all at once.
+``pb_*.hip`` -> ``libpromptcache_blocks.so`` (the bf16 / fp32 building blocks), with it ``py_tensors.cpp`` -> ``_tensors.so`` (host code).  One hipcc per
+translation unit, all at once.
 """
 from __future__ import annotations
 
@@ -46,6 +47,27 @@ def stale(group: str) -> bool:
     return any(os.path.getmtime(d) > os.path.getmtime(lib) for d in deps)
 
 
+def build_tensors() -> None:
+    """``py_tensors.cpp`` -> ``_tensors.so``, host code beside the blocks library.  Where Python's or torch's headers are missing it is left out: the wrappers then look at their
+    tensors in Python."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    lib = os.path.join(PKG, "_tensors.so")
+    tmp = lib + f".{os.getpid()}.tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{d}" for d in (os.path.join(root, "include"), os.path.join(root, "include/torch/csrc/api/include"), sysconfig.get_paths()["include"])),
+           os.path.join(CSRC, "py_tensors.cpp"), "-o", tmp, f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    print("[build]", " ".join(cmd), file=sys.stderr, flush=True)
+    try:
+        subprocess.check_call(cmd, stdout=sys.stderr)
+    except (OSError, subprocess.CalledProcessError) as e:
+        print(f"[build] without _tensors.so: {e}", file=sys.stderr, flush=True)
+        return
+    os.replace(tmp, lib)
+
+
 def build(group: str, force: bool = False) -> str:
     """Build the group's library when it is missing or older than its sources (always with ``force``); returns its path.
     Concurrent callers serialise on a lock file, and the library appears under its name only when it is complete."""
@@ -73,6 +95,7 @@ def build(group: str, force: bool = False) -> str:
         for obj, cmd, proc in jobs:
             if proc.wait() != 0:
                 raise subprocess.CalledProcessError(proc.returncode, cmd)
+        build_tensors()
         tmp = lib + f".{os.getpid()}.tmp"
         link = [hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", *[o for o, _, _ in jobs], "-o", tmp]
         print("[build]", " ".join(link), file=sys.stderr, flush=True)

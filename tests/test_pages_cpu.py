@@ -122,6 +122,42 @@ def test_scratch_of_key_runs():
             B.attn_pages_part(*bad)
 
 
+def test_compiled_looks_are_the_python_ones():
+    """What the compiled helpers accept, return and refuse is what the Python functions of the same names do (on host tensors, device -1)."""
+    tensors = pytest.importorskip("promptcache_amd._tensors")
+    assert tensors.torch_version == torch.__version__.split("+")[0]
+    flat, heads, table, pool = B._looks
+    i32, f32 = torch.arange(60, dtype=torch.int32), torch.ones(60)
+    kc, vc, ks = torch.zeros((3, 2, 16, 32), dtype=torch.int8), torch.zeros((3, 2, 32, 16), dtype=torch.int8), torch.ones((3, 2))
+    e4 = torch.float8_e4m3fn
+    rows = torch.zeros((5, 4, 32), dtype=torch.bfloat16)
+    some = [
+        ("flat", flat, [(t, d, n, dev, "x") for t in (None, i32, i32[7:], i32[::2], i32.view(6, 10).t(), i32[:0], f32, i32.long(), torch.zeros(3, dtype=torch.int32).to_sparse())
+                        for d in (torch.int32, torch.float32) for n in (0, 30, 60, 61) for dev in (-1, 0)]),
+        ("heads", heads, [(t, h, d, dev, "x") for t in (rows, rows[:1], rows[:, :1], rows[::2], rows[:, :, ::2], rows.transpose(0, 1), rows[:0], rows[0], rows.expand(5, 4, 32), f32)
+                          for h in (1, 4, 5) for d in (16, 32) for dev in (-1, 0)]),
+        ("table", table, [(t, n, dev, "x") for t in (i32.view(6, 10), i32.view(6, 10)[:1], i32.view(6, 10)[:, 3:], i32.view(6, 10).t(), i32.view(6, 10)[:0], i32, f32.view(6, 10))
+                          for n in (0, 1, 6, 7) for dev in (-1, 0)]),
+        ("pool", pool, [(a, s, b, s2, dev, "x") for a in (kc, kc.view(e4), kc.float(), kc[:2], kc.transpose(0, 1)) for b in (vc, vc.view(e4), vc[:2], kc)
+                        for s, s2 in ((ks, ks), (ks[:2], ks), (ks, ks.double()), (ks.t(), ks)) for dev in (-1, 0)]),
+    ]
+    taken = 0
+    for name, python, calls in some:
+        for args in calls:
+            got = []
+            for f in (python, getattr(tensors, name)):
+                try:
+                    got.append(f(*args))
+                except Exception as e:                                             # (the same refusal, in the same words)
+                    got.append((type(e), str(e)))
+            assert got[0] == got[1], (name, args, got)
+            taken += not isinstance(got[0], tuple) or not isinstance(got[0][0], type)
+    assert taken > 40
+    for bad in ((), (i32,), (i32, torch.int32, 1, -1, "x", 5), (i32, torch.int32, 1 << 70, -1, "x"), (i32, "int32", 1, -1, "x"), ("x", torch.int32, 1, -1, "x")):
+        with pytest.raises(Exception):
+            tensors.flat(*bad)
+
+
 def test_wrappers_name_what_is_wrong():
     x = torch.zeros((2, 2, 32))
     kc = torch.zeros((4, 2, 16, 32), dtype=torch.int8)
