@@ -41,7 +41,7 @@ struct Query {
             return __uint_as_float(w[e >> 2][e & 3]);
     }
 };
-// .. as halves (PARTS = 2: sums of two) at `to`, the second ones `parts` behind.  THREADS neighbouring lanes hold a row.  -> the power of two that the row was divided by: its largest
+// .. as halves (PARTS = 2: sums of two) at `to` (null: only looked at), the second ones `parts` behind.  THREADS neighbouring lanes, all of them here, hold a row.  -> the power of two that the row was divided by: its largest
 // element becomes 2^14 .. 2^15, and what is 2^-28 of that is still a normal half
 template <typename E, int PARTS, int THREADS>
 __device__ __forceinline__ float as_halves(const Query<E>& q, _Float16* to, int parts) {
@@ -62,6 +62,7 @@ __device__ __forceinline__ float as_halves(const Query<E>& q, _Float16* to, int 
             hi[e] = (_Float16)y;
             if constexpr (PARTS == 2) lo[e] = __builtin_fabsf(y) < __builtin_inff() ? (_Float16)(y - (float)hi[e]) : (_Float16)0.0f;
         }
+        if (!to) continue;
         *reinterpret_cast<h8*>(to + 8 * k) = hi;
         if constexpr (PARTS == 2) *reinterpret_cast<h8*>(to + parts + 8 * k) = lo;
     }
@@ -286,9 +287,9 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(pcb_attn_pages_
             look(s);
             fetch_k(s, 0);
         }
-        if (qc < COLS && qk < 4 * DB) {
-            const float unit2 = as_halves<E, PARTS, TPC>(raw, Qs + qc * QLD + 16 * qk, COLS * QLD);
-            if (qk == 0) unit_s[qc] = F32 ? unit2 * a.scale : unit2 * (a.scale * LOG2E);   // bf16: scores in units of ln 2
+        {
+            const float unit2 = as_halves<E, PARTS, TPC>(raw, qc < COLS && qk < 4 * DB ? Qs + qc * QLD + 16 * qk : nullptr, COLS * QLD);
+            if (qc < COLS && qk == 0) unit_s[qc] = F32 ? unit2 * a.scale : unit2 * (a.scale * LOG2E);   // bf16: scores in units of ln 2
         }
         __syncthreads();
 #pragma unroll

@@ -464,6 +464,20 @@ def test_attention_of_zeros_over_small_keys(T, dtype):
         r.check(r.run(T, scale=scale), scale=scale)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("T", [1, 8, 64])
+@pytest.mark.parametrize("dim", [16, 48, 80, 112, 128, 144, 176, 192, 208, 256])
+def test_attention_of_uneven_queries(T, dtype, dim):
+    """The elements of a row are far apart in size, the largest in any sixteen of them."""
+    r = Requests([300, 40], [9, 7], 6, 3, dim, 32, "int8", dtype, seed=dim)
+    rng = np.random.default_rng(dim)
+    up = np.exp2(rng.integers(-9, 1, (r.q.shape[0], 6, dim // 16)))
+    for i in range(r.q.shape[0]):
+        up[i, np.arange(6), rng.integers(0, dim // 16, 6)] = 4
+    r.q = (r.q.double() * torch.from_numpy(np.repeat(up, 16, axis=2)).to(DEV)).to(r.q.dtype)
+    r.check(r.run(T))
+
+
 @pytest.mark.parametrize("T", [1, 9, 64])
 def test_attention_many_times_alike(T):
     """The same call again and again, among others, on two streams at once: the same bits each time."""
