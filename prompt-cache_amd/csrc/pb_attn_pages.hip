@@ -1,4 +1,4 @@
-// pcb_attn_pages: causal softmax attention over keys and values held in 8 bits in pages, a power-of-two scale for each page and key head.
+// pcb_attn_pages: causal softmax attention over keys and values held in 8 bits in pages, a power-of-two scale for each page and key head.  Here for blocks of 16 or 32 columns.
 //
 // Queries and heads of one key head are COLUMNS of a tile: column = row * (H / Hkv) + head, so a key or value is read and made a number once for all heads that
 // share it.  S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16: codes of both kinds are halves exactly, a query row divided by the power of two
@@ -558,29 +558,34 @@ __global__ __launch_bounds__(256) void attn_pages_merge_kernel(pcb_attn_pages_ar
         if (4 * q + 64 * k < dim) store4(op + 4 * q + 64 * k, v[k][0] * f, v[k][1] * f, v[k][2] * f, v[k][3] * f);
 }
 
-// How a call is cut.  Up to 32 columns a tile (single tokens: any number): in blocks of 16 or 32, the steps of everything shared out to at most two workgroups a CU (three and four:
-// 64 single tokens 54 -> 60 .. 82 us), one for every eight steps (16 over 1 000 keys 15.9 us, for every four 18.6) or four of 32 columns (20 rows over 4 000 22.4, eight 23.9); from
-// 513 tiles on a workgroup a unit.
-// More columns: blocks of 128, in key runs where these are too few to fill the chip twice, of at least 16 steps, 8 where the blocks are less than 128 (always 8: 5 prompts of up to 600
-// rows, fp32, 29.0 -> 33.8 us).  Where that comes to a workgroup a CU at most, heads up to 128, it has eight waves (us, without / with): 216 blocks of 12 heads of 96 27.6 / 21.4, in
-// fp32 39.0 / 32.0; few blocks are then cut for one a CU, not two: 64 rows of 32 heads of 64 over 16 000 keys 31.6 / 25.9, 512 of 16 of 128 over 2 000 37.5 / 31.8 (but 1 500 of 8
-// heads on their own, fp32, 38.4 / 42.7: the last rows' blocks see all keys).
-Plan plan_of(int64_t n_rows, int64_t H, int Hkv, int dim, int n_tiles, int tile_rows, int64_t longest) {
+// Blocks that have columns, at most: tiles need not be full (full: the blocks of all rows, one after the other).
+int64_t units_of(int64_t n_tiles, int64_t Hkv, int64_t cblocks, int64_t full) { return Hkv * (n_tiles * cblocks < n_tiles + full ? n_tiles * cblocks : n_tiles + full); }
+
+// How a call is cut.  In blocks of 16 or 32 columns, the steps of everything shared out to at most two workgroups a CU (three and four: 64 single tokens 54 -> 60 .. 82 us), one for every
+// eight steps (16 over 1 000 keys 15.9 us, for every four 18.6) or four of 32 columns (20 rows over 4 000 22.4, eight 23.9); from 513 tiles on a workgroup a unit.
+// Or, for tiles of more than 32 columns that are work enough, blocks of 128 whose codes are converted once: from this many steps and units' costs on (us, blocks of 32 or 16 / of 128; 32
+// rows of 32 heads over 2 000 keys, then 16 over 8 000): heads of 64 bf16 13.9 / 17.2, 16.7 / 16.5, of 128 17.6 / 22.1, 23.6 / 20.4, fp32 25.1 / 31.3, 37.0 / 29.8; of 192, whose
+// blocks of 128 fill a CU, 17.2 / 34.1, 29.3 / 33.1 (32 requests of 32 rows over 1 000 45.5 / 43.3); of 256 28.2 / 41.2, 46.0 / 40.0.
+// Their key runs where these are too few to fill the chip twice have at least 16 steps, 8 where the blocks are less than 128 (always 8: 5 prompts of up to 600 rows, fp32, 29.0 ->
+// 33.8).  Where that comes to a workgroup a CU at most, heads up to 128, it has eight waves (without / with): 216 blocks of 12 heads of 96 27.6 / 21.4, in fp32 39.0 / 32.0; few blocks
+// are then cut for one a CU, not two: 64 rows of 32 heads of 64 over 16 000 keys 31.6 / 25.9, 512 of 16 of 128 over 2 000 37.5 / 31.8 (but 1 500 of 8 heads on their own, fp32, 38.4 /
+// 42.7: the last rows' blocks see all keys).
+Plan plan_of(bool f32, int64_t n_rows, int64_t H, int Hkv, int dim, int n_tiles, int tile_rows, int64_t longest) {
     Plan p{};
     p.per = (int)(H / Hkv);
     p.magic = p.per > 1 ? (uint32_t)(((1ull << 32) + p.per - 1) / p.per) : 0;
     const int64_t cols = (int64_t)tile_rows * p.per, steps = (longest + 63) / 64 > 0 ? (longest + 63) / 64 : 1;
-    p.cols = tile_rows > 1 && cols > 32 ? MANY_COLS : cols <= 16 || dim > 128 ? 16 : 32;
+    p.cols = cols <= 16 || dim > 128 ? 16 : 32;
+    const int64_t small = units_of(n_tiles, Hkv, (cols + p.cols - 1) / p.cols, n_rows * p.per / p.cols) * (steps + UNIT_STEPS);
+    if (tile_rows > 1 && cols > 32 && small > (dim > 192 ? 2500 : dim > 128 ? 12500 : dim > 64 && f32 ? 1400 : 4200)) p.cols = MANY_COLS;
     p.cblocks = (int)(cols > 1 << 30 ? 1 << 26 : (cols + p.cols - 1) / p.cols);
     int64_t units = (int64_t)n_tiles * Hkv * p.cblocks;
     p.runs = 1, p.run = 1 << 30;
     if (p.cols == MANY_COLS) {
-        // (tiles need not be full: at most this many blocks have columns at all)
-        const int64_t some = Hkv * (n_tiles + n_rows * p.per / MANY_COLS);
-        if (units > some) units = some;
+        units = units_of(n_tiles, Hkv, p.cblocks, n_rows * p.per / MANY_COLS);
         int64_t n = units >= 512 ? 1 : units >= 128 ? (512 + units - 1) / units : (dim <= 128 ? 256 : 512) / units;
-        const int64_t least = units >= 128 ? 16 : 8;                  // steps of a run
-        if (n > (steps + least - 1) / least) n = (steps + least - 1) / least;
+        const int64_t run = units >= 128 ? 16 : 8;                    // the least steps of one
+        if (n > (steps + run - 1) / run) n = (steps + run - 1) / run;
         if (n > 1) p.run = (int)((steps + n - 1) / n), p.runs = (int)((steps + p.run - 1) / p.run);
         // (a workgroup a CU at most: eight waves each)
         p.halves = dim <= 128 && units * p.runs <= 256 && steps > 1 && (int64_t)n_tiles * Hkv * p.cblocks < 1 << 22;
@@ -661,8 +666,9 @@ int dispatch(const pcb_attn_pages_args& a, const Plan& pl, hipStream_t stream) {
 PCB_EXPORT int64_t pcb_attn_pages_part(int32_t n_rows, int32_t H, int32_t Hkv, int32_t dim, int32_t n_tiles, int32_t tile_rows, int32_t longest) {
     PCB_REQUIRE(n_rows >= 0 && dim > 0 && dim <= 256 && longest >= 0 && sizes_ok(H, Hkv, n_tiles, tile_rows), PCB_ERR_ARG, "pcb_attn_pages_part: bad sizes");
     if (n_rows == 0 || n_tiles == 0) return 0;
-    const Plan p = plan_of(n_rows, H, Hkv, dim, n_tiles, tile_rows, longest);
-    return part_floats(p, n_rows, H, dim, n_tiles);
+    const int64_t a = part_floats(plan_of(false, n_rows, H, Hkv, dim, n_tiles, tile_rows, longest), n_rows, H, dim, n_tiles);
+    const int64_t b = part_floats(plan_of(true, n_rows, H, Hkv, dim, n_tiles, tile_rows, longest), n_rows, H, dim, n_tiles);
+    return a > b ? a : b;
 }
 
 PCB_EXPORT int pcb_attn_pages(const pcb_attn_pages_args* a, void* stream) {
@@ -683,9 +689,9 @@ PCB_EXPORT int pcb_attn_pages(const pcb_attn_pages_args* a, void* stream) {
     PCB_REQUIRE(sizes_ok(a->H, a->Hkv, a->n_tiles, a->tile_rows), PCB_ERR_ARG,
                 "pcb_attn_pages: too many tiles, heads or tile rows (heads times tile rows up to 2^19, 2048 query heads a key head)");
     const int64_t longest = a->longest > 0 ? a->longest : (int64_t)a->max_pages * a->page_size;
-    Plan p = plan_of(a->n_rows, a->H, a->Hkv, a->dim, a->n_tiles, a->tile_rows, longest);
+    Plan p = plan_of(a->dtype == PCB_F32, a->n_rows, a->H, a->Hkv, a->dim, a->n_tiles, a->tile_rows, longest);
     if (a->window > 0 && (int64_t)a->window + a->tile_rows + 62 < longest) {   // no tile sees more keys than this: fewer runs, never more scratch
-        const Plan w = plan_of(a->n_rows, a->H, a->Hkv, a->dim, a->n_tiles, a->tile_rows, (int64_t)a->window + a->tile_rows + 62);
+        const Plan w = plan_of(a->dtype == PCB_F32, a->n_rows, a->H, a->Hkv, a->dim, a->n_tiles, a->tile_rows, (int64_t)a->window + a->tile_rows + 62);
         if (part_floats(w, a->n_rows, a->H, a->dim, a->n_tiles) <= part_floats(p, a->n_rows, a->H, a->dim, a->n_tiles)) p = w;
     }
     p.ps = pcb_log2(a->page_size);
