@@ -350,6 +350,35 @@ def test_attention(past, new, H, Hkv, dim, P, T, kind, dtype):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("past, new, H, Hkv, dim, P, T", [x for x in SIZES if x[-1] > 1])
+def test_attention_in_blocks_of_128(past, new, H, Hkv, dim, P, T, kind, dtype):
+    """A bound of the lengths that has short work look like much: blocks of 128 columns where there are more than 32."""
+    r = Requests(past, new, H, Hkv, dim, P, kind, dtype, seed=len(new) + dim)
+    r.check(r.run(T, longest=1 << 22))
+
+
+LONG = [  # work enough for blocks of 128, in key runs or not, of four waves and of eight; the last two: window, sink
+    ([4000], [128], 16, 2, 64, 32, 128, 0, 0), ([9000, 300], [100, 700], 12, 2, 96, 16, 64, 0, 0), ([5000], [900], 16, 4, 128, 64, 128, 0, 1), ([5000], [900], 16, 4, 128, 64, 128, 700, 1),
+    ([2000], [1500], 32, 8, 48, 128, 128, 0, 0), ([3000], [700], 16, 4, 192, 64, 128, 0, 0), ([3000], [300], 8, 2, 256, 32, 100, 0, 0), ([0], [1300], 8, 2, 128, 16, 64, 0, 1),
+    ([700, 5000, 0], [600, 1, 450], 20, 4, 80, 64, 128, 900, 0)]
+
+
+@pytest.mark.parametrize("dtype, kind", [("bf16", "e4m3"), ("f32", "int8"), ("f32", "e4m3")])
+@pytest.mark.parametrize("past, new, H, Hkv, dim, P, T, window, sink", LONG)
+def test_attention_of_much(past, new, H, Hkv, dim, P, T, window, sink, dtype, kind):
+    """Long prompts and questions; two dozen of their rows against the oracle."""
+    r = Requests(past, new, H, Hkv, dim, P, kind, dtype, seed=dim + window)
+    kw = dict(window=window, sink=[0.5 * h - 3 for h in range(H)] if sink else None)
+    got = r.run(T, **kw)
+    n = sum(new)
+    rows = np.unique(np.concatenate([[0, 1, 31, 32, n - 2, n - 1], np.random.default_rng(n).integers(0, n, 18)]))
+    at = torch.from_numpy(rows).to(DEV)
+    r.q, r.seqs, r.pos = r.q[at], r.seqs[rows], r.pos[rows]
+    r.check(got[at], **kw)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
 @pytest.mark.parametrize("window, sink, T", [(1, False, 1), (5, True, 1), (64, True, 16), (65, False, 64), (200, True, 128), (0, True, 128), (100000, False, 33)])
 def test_attention_with_windows_and_sinks(window, sink, T, kind, dtype):
     new = [1, 1, 1] if T == 1 else [3, 130, 40]
