@@ -12,8 +12,8 @@
 // neighbouring codes of a value column, one 16-byte load.  Pages have at least 16 tokens: a lane needs one page number and one pair of scales a step.
 //
 // Bound by the codes' bytes, which are read once, and before them by a chain of loads that each need the one before (tile, length, page number, keys: ~6 us of a launch).  Measured
-// (the launch alone; bf16, 4 heads a key head of 128): 64 single tokens over up to 8 192 keys, 189 MB, 38.6 us = 4.9 TB/s; one over 131 072, 268 MB, 46 us = 5.8 TB/s, 7 more its
-// merge; 27 rows over 8 247 keys of 32 heads, 68 MB, 26.5 us and 5.3: a wave has two steps of its own there.  A copy reaches 4.9 TB/s, a reading stream ~5.9.
+// (the launch alone; bf16, 4 heads a key head of 128): 64 single tokens over up to 8 192 keys, 189 MB, 37.7 us = 5.0 TB/s; one over 131 072, 268 MB, 44.4 us = 6.0 TB/s, 7.4 more its
+// merge; 27 rows over 8 247 keys of 32 heads, 68 MB, 25.5 us and 5.3: a wave has two steps of its own there.  A copy reaches 4.9 TB/s, a reading stream ~5.9.
 #include "pb_attn_pages.h"
 
 namespace {
