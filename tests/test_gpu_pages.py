@@ -529,6 +529,35 @@ def test_attention_many_times_alike(T):
         assert all(torch.equal(o, want[k]) for o in outs[k])
 
 
+@pytest.mark.parametrize("T", [1, 9, 64])
+def test_two_graphs_of_attention_at_once(T):
+    """Two captured calls, replayed at the same time among eager ones: scratch of their own each."""
+    from promptcache_amd import _blocks as B
+    rs = [Requests([4000, 77, 900], [T, T, T], 8, 2, 128, 64, "e4m3", "bf16", seed=s) for s in (1, 2)]
+    made = []
+    for r in rs:
+        args = (r.q, torch.tensor(r.tiles(T), dtype=torch.int32, device=DEV), T, i32(r.kv), *r.device())
+        out = torch.zeros_like(r.q)
+        torch.cuda.synchronize()
+        g, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(g, stream=st):
+            B.attn_pages(*args, out, scale=1.0)
+        made.append((g, st, out, args))
+    first = []
+    for i in range(10):
+        for g, st, out, _ in made:
+            with torch.cuda.stream(st):
+                out.zero_()
+                g.replay()
+        rs[i % 2].run(T)
+        torch.cuda.synchronize()
+        if i == 0:
+            first = [out.clone() for _, _, out, _ in made]
+            for r, out in zip(rs, first):
+                r.check(out)
+        assert all(torch.equal(out, want) for (_, _, out, _), want in zip(made, first))
+
+
 def test_attention_in_a_graph_is_the_eager_one_but_for_its_merge():
     """A captured call merges in a launch of its own: the same sums in the same order of runs, off by roundings of fp32."""
     r = Requests([4000, 700], [1, 1], 8, 2, 128, 64, "e4m3", "f32", seed=3)
