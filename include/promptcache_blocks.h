@@ -941,6 +941,7 @@ int pcb_pages_read(const pcb_pages_rows_args* a, void* stream);
  * {sequence, first position, query rows (<= tile_rows), first flat row}, the granted tiles of pcb_page_tables.  The query at position i sees key j of its
  * sequence iff j <= i, j < kv_len[sequence], window <= 0 or i - j < window, and table[sequence][j / P] is a page of the pool.
  *   out = sum_j e^(scale q.k_j) v_j / (sum_j e^(scale q.k_j) + e^sink[h]),   sink (fp32 [H]) optional; a row that sees nothing: 0
+ * Scores are fp32: of any size that it holds, known to its rounding (the largest of a row wins however large it is; what is nearer to it than fp32's step there may count like it).
  * out may be q, with q's strides.  Query head h reads key head h / (H / Hkv).  scale > 0.  Tiles without rows or of no sequence, and rows outside [0, n_rows), are passed over.
  * longest: an upper bound of kv_len that the host knows (0: max_pages * P, which pcb_attn_pages_part is then given); it decides into how many key runs a tile is
  * cut, whose results need part: pcb_attn_pages_part(...) floats, aligned to 16 bytes.  counters (int32 [512], optional): zero before the first launch that is given them and

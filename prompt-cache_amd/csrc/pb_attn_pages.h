@@ -40,6 +40,13 @@ __device__ __forceinline__ int row_of(const Plan& pl, int x) { return pl.per == 
 template <typename E>
 __device__ __forceinline__ float pow_of(float x) { return __builtin_amdgcn_exp2f(sizeof(E) == 4 ? x * LOG2E : x); }
 
+// Maxima beyond this are far: fp32 numbers there are 2^-3 or more apart, in the end further than e.  Then a weight's exponent is taken from the same rounded number that the maximum was
+// (one fma of the sum of products, less M: the largest is 0 exactly), not from the exact product less another rounding: half a step of M would make the largest weight more than a
+// half holds, or 0.  Up to it the exponent is off by 2^-3 at most, of numerator and denominator alike.
+constexpr float FAR = 1048576.0f;
+// .. such a sum of products, in units of 1: what it is above M, less ln vs, which the exponent gets again
+__device__ __forceinline__ float above(float s, float f, float lv, float M) { return __builtin_fmaf(s, f, lv) - M - lv; }
+
 // What a sum of products of a query and a key stands for.  Above 0 and finite whatever the two are (a row of zeros over the smallest scale would give 0, and -infinity, a key that is
 // not seen, times 0 is no number); sums that this changes are 0 or too small to count, or beyond all numbers
 __device__ __forceinline__ float score_unit(float qs, float ks) { return __builtin_fminf(__builtin_fmaxf(qs * ks, 1.17549435e-38f), 3.40282347e38f); }

@@ -76,11 +76,17 @@ __device__ __forceinline__ void weights(f4 (&acc)[4], float f, float vs, float& 
     float top = NEG;
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, acc[i >> 2][i & 3]);
-    const float lvs = exp_of(vs);
-    top = max4(top * f + (PARTS == 2 ? lvs * 0.693147181f : lvs));    // (f > 0)
-    const float M_new = fmaxf(M, top), M_use = M_new == NEG ? 0.0f : M_new;
+    const float lvs = exp_of(vs), lv = PARTS == 2 ? lvs * 0.693147181f : lvs;
+    top = max4(__builtin_fmaf(top, f, lv));                           // (f > 0)
+    const float M_new = fmaxf(M, top);
+    float M_use = M_new == NEG ? 0.0f : M_new;
     alpha = pow_of<E>(M - M_use);
     M = M_new;
+    if (__builtin_expect(__builtin_fabsf(M_use) > FAR, 0)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i >> 2][i & 3] = above(acc[i >> 2][i & 3], f, lv, M_use);
+        f = 1.0f, M_use = 0.0f;
+    }
     float sum = 0.0f;
     if constexpr (PARTS == 1) {
         // vs and 2^14 inside the exponent, out of the sum again: all powers of two

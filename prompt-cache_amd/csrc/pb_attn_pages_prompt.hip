@@ -215,11 +215,22 @@ __global__ __launch_bounds__(256 * KS, KS == 1 && sizeof(E) == 2 && ND <= 6 ? 2 
                 float m = acc[q >> 1][8 * (q & 1)];
 #pragma unroll
                 for (int e = 1; e < 8; ++e) m = fmaxf(m, acc[q >> 1][8 * (q & 1) + e]);
-                top = fmaxf(top, m * f[q] + (F32 ? exp_of(vs[q]) * 0.693147181f : exp_of(vs[q])));
+                top = fmaxf(top, __builtin_fmaf(m, f[q], F32 ? exp_of(vs[q]) * 0.693147181f : exp_of(vs[q])));
             }
             top = max2(top);
-            const float M_new = fmaxf(M, top), M_use = M_new == NEG ? 0.0f : M_new;
+            const float M_new = fmaxf(M, top);
+            float M_use = M_new == NEG ? 0.0f : M_new;
             const float alpha = pow_of<E>(M - M_use);
+            if (__builtin_expect(__builtin_fabsf(M_use) > FAR, 0)) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        acc[q >> 1][8 * (q & 1) + e] = above(acc[q >> 1][8 * (q & 1) + e], f[q], F32 ? exp_of(vs[q]) * 0.693147181f : exp_of(vs[q]), M_use);
+                    f[q] = 1.0f;
+                }
+                M_use = 0.0f;
+            }
             h8 wf[PARTS][4];
             float sum = 0.0f;
 #pragma unroll
