@@ -570,8 +570,10 @@ int64_t units_of(int64_t n_tiles, int64_t Hkv, int64_t cblocks, int64_t full) { 
 // How a call is cut.  In blocks of 16 or 32 columns, the steps of everything shared out to at most two workgroups a CU (three and four: 64 single tokens 54 -> 60 .. 82 us), one for every
 // eight steps (16 over 1 000 keys 15.9 us, for every four 18.6) or four of 32 columns (20 rows over 4 000 22.4, eight 23.9); from 513 tiles on a workgroup a unit.
 // Or, for tiles of more than 32 columns that are work enough, blocks of 128 whose codes are converted once: from this many steps and units' costs on (us, blocks of 32 or 16 / of 128; 32
-// rows of 32 heads over 2 000 keys, then 16 over 8 000): heads of 64 bf16 13.9 / 17.2, 16.7 / 16.5, of 128 17.6 / 22.1, 23.6 / 20.4, fp32 25.1 / 31.3, 37.0 / 29.8; of 192, whose
+// rows of 32 heads over 2 000 keys, then 16 over 8 000): heads of 64 bf16 13.9 / 17.2, 16.7 / 16.5, of 128 17.5 / 22.2, 23.5 / 20.2, fp32 25.1 / 31.3, 37.0 / 29.8; of 192, whose
 // blocks of 128 fill a CU, 17.2 / 34.1, 29.3 / 33.1 (32 requests of 32 rows over 1 000 45.5 / 43.3); of 256 28.2 / 41.2, 46.0 / 40.0.
+// bf16 heads of 128 also hang on how long the units are.  64 steps and more, costs of 1 896 18.9 / 24.1, 2 144 23.7 / 21.6, 2 336 24.8 / 22.3, 2 472 22.6 / 24.6, 3 132 24.3 / 23.1, 3 264
+// 24.4 / 21.8, 4 176 26.3 / 23.2; shorter ones, 2 304 19.4 / 21.3, 2 560 21.3 / 21.5, 2 880 19.6 / 20.3, 3 072 20.3 / 21.8, 3 520 11.8 / 13.1.
 // Their key runs where these are too few to fill the chip twice have at least 16 steps, 8 where the blocks are less than 128 (always 8: 5 prompts of up to 600 rows, fp32, 29.0 ->
 // 33.8).  Where that comes to a workgroup a CU at most, heads up to 128, it has eight waves (without / with): 216 blocks of 12 heads of 96 27.6 / 21.4, in fp32 39.0 / 32.0; few blocks
 // are then cut for one a CU, not two: 64 rows of 32 heads of 64 over 16 000 keys 31.6 / 25.9, 512 of 16 of 128 over 2 000 37.5 / 31.8 (but 1 500 of 8 heads on their own, fp32, 38.4 /
@@ -583,7 +585,8 @@ Plan plan_of(bool f32, int64_t n_rows, int64_t H, int Hkv, int dim, int n_tiles,
     const int64_t cols = (int64_t)tile_rows * p.per, steps = (longest + 63) / 64 > 0 ? (longest + 63) / 64 : 1;
     p.cols = cols <= 16 || dim > 128 ? 16 : 32;
     const int64_t small = units_of(n_tiles, Hkv, (cols + p.cols - 1) / p.cols, n_rows * p.per / p.cols) * (steps + UNIT_STEPS);
-    if (tile_rows > 1 && cols > 32 && small > (dim > 192 ? 2500 : dim > 128 ? 12500 : dim > 64 && f32 ? 1400 : 4200)) p.cols = MANY_COLS;
+    const int64_t much = dim > 192 ? 2500 : dim > 128 ? 12500 : dim <= 64 ? 4200 : f32 ? 1400 : steps >= 64 ? 2000 : 4200;
+    if (tile_rows > 1 && cols > 32 && small > much) p.cols = MANY_COLS;
     p.cblocks = (int)(cols > 1 << 30 ? 1 << 26 : (cols + p.cols - 1) / p.cols);
     int64_t units = (int64_t)n_tiles * Hkv * p.cblocks;
     p.runs = 1, p.run = 1 << 30;
