@@ -909,6 +909,9 @@ typedef struct pcb_page_tables_args {
     int32_t* status;
 } pcb_page_tables_args;
 int pcb_page_tables(const pcb_page_tables_args* a, void* stream);
+/* keep [n_seqs] for pcb_page_tables where sequences share pages, which are then their first ones: of a sequence that is over, how many of its first pages one that goes on, or that is over
+ * before it (in order), has too; 0 for the others.  So a page goes back with the last sequence that has it, whichever that is. */
+int pcb_pages_kept(int32_t n_seqs, const int32_t* cached, const int32_t* brings, const int32_t* table, int64_t ld_table, int32_t max_pages, int32_t page_size, int32_t* keep, void* stream);
 
 /* New rows into the pool, and rows of it back.  Row r of k and v (E, head h at r * ldk + h * k_head_stride, likewise v; 16-byte pieces) belongs to row_slot[r];
  * rows whose slot is below zero or outside the pool are passed over.

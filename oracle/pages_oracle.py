@@ -127,6 +127,23 @@ def tables(cached, brings, table, P, rows, *, tile_rows=1, n_tiles=0, ring=None,
     return {k: np.array(v) for k, v in out.items()}
 
 
+def kept(cached, brings, table, P):
+    """Of each sequence that is over, how many of its first pages one that goes on, or one before it that is over, has too (0: it goes on)."""
+    table = np.asarray(table)
+    pages = [[int(p) for p in table[s, :min(-(-max(int(c), 0) // P), table.shape[1])]] for s, c in enumerate(cached)]
+    out = []
+    for s, mine in enumerate(pages):
+        most = 0
+        for t, other in enumerate(pages):
+            if brings[s] < 0 and t != s and (brings[t] >= 0 or t < s):
+                n = 0
+                while n < min(len(mine), len(other)) and mine[n] == other[n]:
+                    n += 1
+                most = max(most, n)
+        out.append(most)
+    return np.array(out)
+
+
 def attend(q, seqs, positions, kv_len, table, kcodes, kscale, vcodes, vscale, P, kind, scale, window=0, sink=None):
     """Rows ``q`` [rows, H, dim] at ``positions`` of ``seqs`` (below zero: the row is left out, zeros); codes uint8, values' [pages, Hkv, dim, P]."""
     q = np.asarray(q, dtype=np.float64)

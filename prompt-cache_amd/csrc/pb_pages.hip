@@ -163,6 +163,34 @@ __global__ __launch_bounds__(NT) void page_tables_kernel(pcb_page_tables_args a,
     }
 }
 
+// A wave a sequence; one that is over looks at the others, a lane each: pages are equal up to some place and nowhere behind it, so the place is found by halving.
+__global__ __launch_bounds__(256) void pages_kept_kernel(int n_seqs, const int32_t* cached, const int32_t* brings, const int32_t* table, int64_t ld_table, int max_pages, int ps, int32_t* keep) {
+    const int lane = threadIdx.x & 63, s = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (s >= n_seqs) return;
+    auto pages_of = [&](int t) { return (int)min(((int64_t)max(cached[t], 0) + (1 << ps) - 1) >> ps, (int64_t)max_pages); };
+    int most = 0;
+    if (brings[s] < 0) {
+        const int32_t* mine = table + (int64_t)s * ld_table;
+        const int have = pages_of(s);
+        for (int t = lane; t < n_seqs && have > 0; t += 64) {
+            if (t == s || (brings[t] < 0 && t > s)) continue;
+            const int32_t* other = table + (int64_t)t * ld_table;
+            int lo = most, hi = min(have, pages_of(t));               // lo pages are equal, or the other way to as many has been found
+            while (lo < hi) {
+                const int mid = lo + (hi - lo + 1) / 2;
+                if (mine[mid - 1] == other[mid - 1])
+                    lo = mid;
+                else
+                    hi = mid - 1;
+            }
+            most = lo;
+        }
+#pragma unroll
+        for (int x = 32; x > 0; x >>= 1) most = max(most, __shfl_xor(most, x, 64));
+    }
+    if (lane == 0) keep[s] = most;
+}
+
 // ---- rows into pages ------------------------------------------------------------------------------------------------------------------------
 // sixteen bytes of a row, CE elements
 template <typename E>
@@ -504,6 +532,15 @@ PCB_EXPORT int pcb_page_tables(const pcb_page_tables_args* a, void* stream) {
     else
         hipLaunchKernelGGL(page_tables_kernel<1024>, dim3(groups), dim3(1024), 0, (hipStream_t)stream, b, ps);
     return pcb_check_launch("page_tables_kernel");
+}
+
+PCB_EXPORT int pcb_pages_kept(int32_t n_seqs, const int32_t* cached, const int32_t* brings, const int32_t* table, int64_t ld_table, int32_t max_pages, int32_t page_size, int32_t* keep,
+                              void* stream) {
+    PCB_REQUIRE(n_seqs > 0 && max_pages > 0 && ld_table >= max_pages && pcb_page_size_ok(page_size) && (int64_t)n_seqs * max_pages < 0x7fffffff, PCB_ERR_ARG,
+                "pcb_pages_kept: bad sizes (pages of 16, 32, 64 or 128 tokens)");
+    PCB_REQUIRE(cached && brings && table && keep, PCB_ERR_ARG, "pcb_pages_kept: null pointer");
+    hipLaunchKernelGGL(pages_kept_kernel, dim3(pcb_ceil_div(n_seqs, 4)), dim3(256), 0, (hipStream_t)stream, n_seqs, cached, brings, table, ld_table, max_pages, pcb_log2(page_size), keep);
+    return pcb_check_launch("pages_kept_kernel");
 }
 
 #define PCB_PAGES_LAUNCH2(KERNEL, E, CODE, PAST, GRID, ...)                                                                        \

@@ -293,6 +293,7 @@ SIGNATURES = {
     "pcb_rec_step_fits": (C.c_int32, [_i32, _i32]),
     "pcb_rec_step": (C.c_int, [C.POINTER(RecArgs), _vp]),
     "pcb_page_tables": (C.c_int, [_vp, _vp]),
+    "pcb_pages_kept": (C.c_int, [_i32, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp]),
     "pcb_pages_append": (C.c_int, [_vp, _vp]),
     "pcb_pages_read": (C.c_int, [_vp, _vp]),
     "pcb_attn_pages_part": (_i64, [_i32] * 7),
@@ -1285,6 +1286,18 @@ def page_tables(cached: torch.Tensor, brings: torch.Tensor, table: torch.Tensor,
     rc = (_lib or load()).pcb_page_tables(a, _raw_stream(dev))
     if rc:
         check(rc, "pcb_page_tables")
+
+
+def pages_kept(cached: torch.Tensor, brings: torch.Tensor, table: torch.Tensor, page_size: int, keep: torch.Tensor) -> None:
+    """``keep`` int32 [n] for ``page_tables`` where sequences begin with the same pages: of each that is over, how many of its first pages a sequence that goes on, or that is over
+    before it, has too."""
+    n = cached.numel()
+    dev = _device_of(cached, "pages_kept cached")
+    tab, ld, pages = _table(table, n, dev, "pages_kept")
+    rc = (_lib or load()).pcb_pages_kept(n, _flat(cached, _I32, n, dev, "cached"), _flat(brings, _I32, n, dev, "brings"), tab, ld, pages, page_size, _flat(keep, _I32, n, dev, "keep"),
+                                         _raw_stream(dev))
+    if rc:
+        check(rc, "pcb_pages_kept")
 
 
 def _pages_rows(name: str, k, v, row_slot, kcodes, kscale, vcodes, vscale) -> None:

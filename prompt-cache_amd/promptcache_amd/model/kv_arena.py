@@ -488,10 +488,12 @@ class PageCache:
         s.row_slot, s.row_seq, s.row_pos = self._buf("slot", (rows,), torch.int64), self._buf("seq", (rows,), torch.int32), self._buf("pos", (rows,), torch.int32)
         s.row_start, s.status = self._buf("start", (self.seqs + 1,), torch.int32), self._buf("status", (2,), torch.int32)
         s.tiles = self._buf("tiles", (self.seqs + rows // tile_rows, 4), torch.int32)
-        B.page_tables(self.cached, brings, self.table, self.page_size, row_slot=s.row_slot, kv_len=self.cached, row_start=s.row_start, row_seq=s.row_seq, row_pos=s.row_pos,
-                      tiles=s.tiles, tile_rows=tile_rows, status=s.status, ring=self.ring, ring_state=self.ring_state, ring_out=self.ring_state, keep=self.keep)
+        keep = None
         if self._shared or self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():   # (a replay may follow a later `share`)
-            self.keep.masked_fill_(brings < 0, 0)                 # (whoever takes the sequence's place owns all of its pages)
+            keep = self.keep
+            B.pages_kept(self.cached, brings, self.table, self.page_size, keep)
+        B.page_tables(self.cached, brings, self.table, self.page_size, row_slot=s.row_slot, kv_len=self.cached, row_start=s.row_start, row_seq=s.row_seq, row_pos=s.row_pos,
+                      tiles=s.tiles, tile_rows=tile_rows, status=s.status, ring=self.ring, ring_state=self.ring_state, ring_out=self.ring_state, keep=keep)
         s.kv_len = self.cached
         return s
 
@@ -518,15 +520,14 @@ class PageCache:
         return out
 
     def share(self, source: int, target: int, tokens: int) -> None:
-        """Sequence ``target`` starts with the first ``tokens`` tokens of ``source``, in the same pages: whole pages only, nobody appends to them.  ``target`` holds nothing
-        before; ``source`` stays until ``target`` is over (the pages are its own, and are free when it is over)."""
+        """Sequence ``target``, which holds nothing before, starts with the first ``tokens`` tokens of ``source``, in the same pages: whole pages only, nobody appends to
+        them.  Either may be over first: a page is free when the last sequence that has it is over."""
         if tokens < 0 or tokens % self.page_size or tokens > self.max_pages * self.page_size or source == target or \
                 not (0 <= source < self.seqs and 0 <= target < self.seqs):
             raise ValueError(f"sequences share whole pages of {self.page_size} tokens")
         n = tokens // self.page_size
         self.table[target, :n].copy_(self.table[source, :n])
         self.cached[target:target + 1].fill_(tokens)
-        self.keep[target:target + 1].fill_(n)
         self._shared = True
 
     def read(self, layer: int, slots: torch.Tensor, dtype=torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
