@@ -520,14 +520,14 @@ class PageCache:
         return out
 
     def share(self, source: int, target: int, tokens: int) -> None:
-        """Sequence ``target``, which holds nothing before, starts with the first ``tokens`` tokens of ``source``, in the same pages: whole pages only, nobody appends to
-        them.  Either may be over first: a page is free when the last sequence that has it is over."""
+        """Sequence ``target``, which holds nothing before, starts with the first ``tokens`` tokens of ``source`` (as far as that holds whole pages of them), in the same pages: nobody
+        appends to those.  Either may be over first: a page is free when the last sequence that has it is over."""
         if tokens < 0 or tokens % self.page_size or tokens > self.max_pages * self.page_size or source == target or \
                 not (0 <= source < self.seqs and 0 <= target < self.seqs):
             raise ValueError(f"sequences share whole pages of {self.page_size} tokens")
         n = tokens // self.page_size
         self.table[target, :n].copy_(self.table[source, :n])
-        self.cached[target:target + 1].fill_(tokens)
+        self.cached[target:target + 1].copy_((self.cached[source:source + 1] & -self.page_size).clamp_(0, tokens))   # (table entries behind what a sequence holds are old ones)
         self._shared = True
 
     def read(self, layer: int, slots: torch.Tensor, dtype=torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:

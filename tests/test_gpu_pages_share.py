@@ -120,6 +120,20 @@ def test_many_that_begin_alike_end_in_any_order():
     assert a.cache.ring_state.tolist()[1] == 30
 
 
+def test_a_share_of_more_than_there_is():
+    """The whole pages that the source holds: what its table has behind them are pages of others."""
+    a = Story(3, 12, seed=2)
+    a.step([0, 60, 0])
+    a.step([20, -1, 0])
+    a.step([1, 40, 0])                                                # (1's table still names a fourth page, from before)
+    a.step([-1, 1, 0])
+    a.share(1, 2, 64)                                                 # 41 tokens: two pages
+    a.step([30, 1, 1])
+    a.step([-1, 1, 1])
+    a.step([0, -1, 30])
+    a.step([0, 0, -1])
+
+
 def test_a_captured_step_whose_source_is_over_first():
     from promptcache_amd.model.kv_arena import PageCache
     cache = PageCache([(1, 16)], 3, 12, DEV, page_size=16)
