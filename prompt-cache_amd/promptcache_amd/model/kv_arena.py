@@ -476,10 +476,12 @@ class PageCache:
         return t[:n].view(shape)
 
     def begin(self, brings, rows: int, *, tile_rows: int = 1, longest: int = 0) -> PageStep:
-        """Tables of a step.  ``brings``: new tokens of every sequence (0: none, -1: the sequence is over and its pages are free), an int32 device tensor or numbers;
-        ``rows``: at least their sum (rows behind it have no slot); ``longest``: an upper bound of the lengths after the step, 0 where the host knows none."""
+        """Tables of a step.  ``brings``: new tokens of every sequence (0: none, -1: the sequence is over and its pages are free), an int32 device tensor or numbers (in a
+        capture: a tensor); ``rows``: at least their sum (rows behind it have no slot); ``longest``: an upper bound of the lengths after the step, 0 where the host knows none."""
         from .. import _blocks as B
         if not isinstance(brings, torch.Tensor):
+            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():   # (a replay would copy from pinned memory that is another's by then)
+                raise RuntimeError("a captured step takes its new tokens from a device tensor")
             brings = uploaded(list(brings), torch.int32, self.device)
         if brings.numel() != self.seqs or rows < 0 or tile_rows < 1:
             raise ValueError(f"a step names the new tokens of all {self.seqs} sequences, its rows and tiles of at least one row")

@@ -1,7 +1,8 @@
-"""Pages that sequences share, without a GPU: the oracle, and what the entry point refuses."""
+"""Pages that sequences share, without a GPU: the oracle, and what the entry point and the cache refuse."""
 import ctypes as C
 
 import pytest
+import torch
 
 from oracle import pages_oracle as O
 from promptcache_amd import _blocks as B
@@ -24,3 +25,16 @@ def test_what_pages_kept_refuses(bad):
     lib = B.load()
     assert lib.pcb_pages_kept(a["n"], a["cached"], a["brings"], a["table"], C.c_int64(a["ld"]), a["wide"], a["P"], a["keep"], None) == -2001
     assert b"pcb_pages_kept" in lib.pcb_last_error_string()
+
+
+def test_a_captured_step_takes_no_host_numbers(monkeypatch):
+    """Its copy would run again with every replay, out of memory that is another's by then."""
+    from promptcache_amd.model import kv_arena
+    cache = kv_arena.PageCache([(1, 16)], 2, 4, "cpu", page_size=16)
+    cache.device = torch.device("cuda")
+    copied = []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(kv_arena, "uploaded", lambda *a: copied.append(a))
+    with pytest.raises(Exception) as e:
+        cache.begin([1, 1], 2)
+    assert not copied and e.type is RuntimeError, e.value
