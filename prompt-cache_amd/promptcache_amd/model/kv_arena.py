@@ -541,8 +541,9 @@ class PageCache:
         return k, v
 
     def rows(self, layer: int, seq: int, tokens: int, dtype=torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
-        """The first ``tokens`` tokens of a sequence as dense rows ``[tokens, heads, dim]``."""
+        """The first ``tokens`` tokens of a sequence as dense rows ``[tokens, heads, dim]``; zeros behind the last one that it holds."""
         from .. import _blocks as B
         slots = torch.empty(tokens, dtype=torch.int64, device=self.device)
-        B.page_tables(torch.zeros(1, dtype=torch.int32, device=self.device), uploaded([tokens], torch.int32, self.device), self.table[seq:seq + 1], self.page_size, row_slot=slots)
+        held = self.cached[seq:seq + 1].clamp(max=tokens)            # (table entries behind it are old ones)
+        B.page_tables(torch.zeros_like(held), held, self.table[seq:seq + 1], self.page_size, row_slot=slots)
         return self.read(layer, slots, dtype)

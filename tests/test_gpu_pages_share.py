@@ -159,3 +159,15 @@ def test_a_captured_step_whose_source_is_over_first():
     assert first[1] == first[0] and first[2][:2] == first[0][:2]
     assert step(60, -1, 0) == 6 - 4 + 2                               # 1's own one, and the third that only it had left
     assert step(0, 0, -1) == 8 and step(-1, 0, 0) == 12 and sorted(cache.ring.tolist()) == list(range(12))
+
+
+def test_rows_behind_what_a_sequence_holds():
+    """Zeros: the table's entries there are pages that others have by now."""
+    a = Story(2, 5, seed=3)
+    a.step([40, 0])
+    a.step([-1, 30])
+    a.step([3, 30])                                                   # (1 has 0's former pages)
+    for n in (1, 3, 4, 16, 17, 48, 100):
+        k, v = a.cache.rows(0, 0, n, torch.float32)
+        assert k.shape == v.shape == (n, 2, 32)
+        assert bool((k[:3] != 0).any()) and not bool((k[3:] != 0).any()) and not bool((v[3:] != 0).any()), n
