@@ -5,6 +5,7 @@ and a failing call raises ``RuntimeError`` with the library's own message.
 from __future__ import annotations
 
 import ctypes as C
+import importlib
 import struct
 from typing import Optional
 
@@ -307,7 +308,7 @@ def lib_path() -> str:
 
 def load(build_missing: bool = True) -> C.CDLL:
     """Load the library (once); a missing one is compiled first unless ``build_missing`` is off."""
-    global _lib
+    global _lib, _compiled
     if _lib is not None:
         return _lib
     import os
@@ -321,6 +322,8 @@ def load(build_missing: bool = True) -> C.CDLL:
         fn.restype, fn.argtypes = res, args
     if lib.pcb_version() != ABI_VERSION:
         raise RuntimeError("libpromptcache_blocks.so: ABI version mismatch (rebuild it)")
+    if build_missing and not _compiled:
+        _compiled = _compile_looks()
     _lib = lib
     return lib
 
@@ -1258,13 +1261,33 @@ def _table(table: torch.Tensor, n: int, dev: int, what: str):
 
 
 _looks = (_flat, _heads, _table, _pool)
-try:                                                               # (the same looks in a call each, where they were compiled for this torch: 2 to 4 us of a call's 9 to 12)
-    from . import _tensors
-    if _tensors.torch_version == torch.__version__.split("+")[0]:
-        _tensors.behind(*_looks)
-        _flat, _heads, _table, _pool = _tensors.flat, _tensors.heads, _tensors.table, _tensors.pool
-except ImportError:
-    pass
+
+
+def _bind_looks() -> bool:
+    """The same looks in a call each (2 to 4 us of a call's 9 to 12), if they were compiled, and for this torch."""
+    global _flat, _heads, _table, _pool
+    try:
+        importlib.invalidate_caches()
+        t = importlib.import_module(__package__ + "._tensors")
+    except ImportError:
+        return False
+    if t.torch_version != torch.__version__.split("+")[0]:
+        return False
+    t.behind(*_looks)
+    _flat, _heads, _table, _pool = t.flat, t.heads, t.table, t.pool
+    return True
+
+
+def _compile_looks() -> bool:
+    """.. compiled where they were not (Another torch's that are loaded stay loaded: the next process finds the new ones.)."""
+    try:
+        _buildlib.renew_tensors()
+    except OSError:                                                # (nowhere to put them)
+        return False
+    return _bind_looks()
+
+
+_compiled = _bind_looks()
 
 _tables_args, _rows_args, _attn_args = _packed(PageTablesArgs), _packed(PagesRowsArgs), _packed(AttnPagesArgs)
 

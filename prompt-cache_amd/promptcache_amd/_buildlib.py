@@ -7,6 +7,7 @@ translation unit, all at once.
 """
 from __future__ import annotations
 
+import contextlib
 import fcntl
 import glob
 import os
@@ -47,6 +48,36 @@ def stale(group: str) -> bool:
     return any(os.path.getmtime(d) > os.path.getmtime(lib) for d in deps)
 
 
+def tensors_path() -> str:
+    return os.path.join(PKG, "_tensors.so")
+
+
+def tensors_stale() -> bool:
+    """Whether ``_tensors.so`` is missing or older than its source.  (Whether it is this torch's: whoever loads it sees.)"""
+    lib = tensors_path()
+    return not os.path.exists(lib) or os.path.getmtime(os.path.join(CSRC, "py_tensors.cpp")) > os.path.getmtime(lib)
+
+
+@contextlib.contextmanager
+def _locked(group: str):
+    """Concurrent builders of a group, one after the other."""
+    objdir = os.path.join(CSRC, "_build")
+    os.makedirs(objdir, exist_ok=True)
+    with open(os.path.join(objdir, f".{group}.lock"), "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        yield objdir
+
+
+def renew_tensors() -> None:
+    """``_tensors.so`` anew, unless somebody else has just made it."""
+    def made():
+        return os.stat(tensors_path()).st_mtime_ns if os.path.exists(tensors_path()) else None
+    seen = made()
+    with _locked("blocks"):
+        if made() == seen:
+            build_tensors()
+
+
 def build_tensors() -> None:
     """``py_tensors.cpp`` -> ``_tensors.so``, host code beside the blocks library.  Where Python's or torch's headers are missing it is left out: the wrappers then look at their
     tensors in Python."""
@@ -54,7 +85,7 @@ def build_tensors() -> None:
 
     import torch
     root = os.path.dirname(torch.__file__)
-    lib = os.path.join(PKG, "_tensors.so")
+    lib = tensors_path()
     tmp = lib + f".{os.getpid()}.tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f"-I{d}" for d in (os.path.join(root, "include"), os.path.join(root, "include/torch/csrc/api/include"), sysconfig.get_paths()["include"])),
@@ -73,10 +104,9 @@ def build(group: str, force: bool = False) -> str:
     Concurrent callers serialise on a lock file, and the library appears under its name only when it is complete."""
     pattern, _, extra = GROUPS[group]
     lib = lib_path(group)
-    objdir = os.path.join(CSRC, "_build")
-    os.makedirs(objdir, exist_ok=True)
-    with open(os.path.join(objdir, f".{group}.lock"), "w") as lock:
-        fcntl.flock(lock, fcntl.LOCK_EX)
+    with _locked(group) as objdir:
+        if group == "blocks" and (force or tensors_stale()):
+            build_tensors()
         if not force and not stale(group):
             return lib
         srcs = sorted(glob.glob(os.path.join(CSRC, pattern)))
@@ -95,7 +125,6 @@ def build(group: str, force: bool = False) -> str:
         for obj, cmd, proc in jobs:
             if proc.wait() != 0:
                 raise subprocess.CalledProcessError(proc.returncode, cmd)
-        build_tensors()
         tmp = lib + f".{os.getpid()}.tmp"
         link = [hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", *[o for o, _, _ in jobs], "-o", tmp]
         print("[build]", " ".join(link), file=sys.stderr, flush=True)
