@@ -5,7 +5,7 @@
 // latency of the loads and of three scans one after the other, so a batch of one chunk and few rows is one workgroup.  Measured: 64 sequences of one token 6.7 us, 517 sequences
 // and 95 700 rows 11.0.
 //
-// pcb_pages_append / pcb_pages_read: a wave takes the rows of one page (16 keys of it when reading) of one head, keys or values, by itself: no LDS, no barrier, and
+// pcb_pages_append / pcb_pages_read: a wave takes the rows of one page (reading: 4 to 32 rows, of any pages) of one head, keys or values, by itself: no LDS, no barrier, and
 // the maximum of a page is a wave's reduction.  Both are bound by memory: rows in and codes out, each once.  Measured: 19 325 rows of 8 heads of 128 in and out again, 238 MB,
 // 58 us = 4.1 TB/s; 8 247 rows of 32 heads out, 203 MB, 32.5 us = 6.2 TB/s (a copy reaches 4.9: here twice as much is written as read).
 #include "pb_pages.h"
@@ -259,7 +259,8 @@ struct RowsView {
 //
 // A lane takes sixteen rows, those whose places share a multiple of 16, and sixteen bytes of each: the maximum, a key row's codes and a value column's sixteen codes (one
 // store) all come out of the same registers, and a page of 64 rows of 128 bf16 elements is one such load for the wave, read once.  (Rows first for the maximum, then again for
-// the codes, value columns a row a lane at a time: 55 us for 19 325 rows of 8 heads.)  Larger pages are read twice, the second time from the caches.
+// the codes, value columns a row a lane at a time: 55 us for 19 325 rows of 8 heads.)  Larger pages are read twice, the second time as far as the caches held them: 9 600 rows of
+// 8 x 128 in fp32 54 us = 1.8 TB/s, in pages of 128 93 = 1.1; bf16 in pages of 128 1.9, of 16, which leave lanes idle, 2.5, of 32 3.6, of 64 4.1.
 template <typename E, int CODE, bool PAST, bool VALUES>
 __device__ void append_run(const pcb_pages_rows_args& a, const RowsView& v, int64_t r0, int n, int64_t s0, int off_min, bool even, int h, int lane) {
     constexpr int CE = Piece<E>::CE;
@@ -567,7 +568,10 @@ PCB_EXPORT int pcb_pages_kept(int32_t n_seqs, const int32_t* cached, const int32
 static bool past_caches(const pcb_pages_rows_args* a) {
     return (int64_t)a->n_rows * a->Hkv * a->dim * (a->dtype == PCB_BF16 ? 4 : 8) > (int64_t)32 << 20;
 }
-// rows that a wave looks at: as many as leave the chip's 1024 SIMDs two waves each or more, at most 64
+// .. but not the rows of an append whose pages are more than one load of a wave, which are read twice (19 325 rows of 8 heads of 128, fp32 68.2 -> 62.7, bf16 in pages of 128 65.3 -> 61.8;
+// 6 000 of 8 x 256, fp32, pages of 128 116.2 -> 104.7)
+static bool read_once(const pcb_pages_rows_args* a) { return a->page_size / 16 * a->dim / (a->dtype == PCB_BF16 ? 8 : 4) <= 64; }
+// rows that a wave looks at: as many as leave the chip's 1024 SIMDs four waves each or more, keys' and values' together, at most 64
 static int window(int n_rows, int Hkv, int least, int most) {
     int w = least;
     while (w < most && (int64_t)n_rows * Hkv * 2 / (2 * w) >= 4096) w *= 2;
@@ -581,7 +585,7 @@ PCB_EXPORT int pcb_pages_append(const pcb_pages_rows_args* a, void* stream) {
     const int win = window(a->n_rows, a->Hkv, 1, a->page_size < 64 ? 32 : 64);   // (rows of different requests side by side; prompts: a page or two start in a window)
     const int64_t waves = ((int64_t)a->n_rows + win - 1) / win * a->Hkv;
     const dim3 grid((unsigned)((waves + 3) / 4), 2);
-    PCB_PAGES_LAUNCH(pages_append_kernel, past_caches(a), grid, v, win);
+    PCB_PAGES_LAUNCH(pages_append_kernel, past_caches(a) && read_once(a), grid, v, win);
     return pcb_check_launch("pages_append_kernel");
 }
 
