@@ -4,6 +4,11 @@
 // share it.  S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16: codes of both kinds are halves exactly, a query row divided by the power of two
 // of its largest element is (bf16) or is as the sum of two halves (fp32, 22 bits), and softmax weights are 11 bits (fp32: 22).  All sums are fp32.
 //
+// A bf16 row's weights enter the second product as one half.  The attention of this library whose operands are bf16 has them as a pair, 17 bits, for one bf16 has 8, no more than the
+// result; a half's 11 move a result by 1.0 to 3.0e-4 of its norm, where its own rounding is 1.6e-3, and its distance from 64 bits by nothing that shows: 64 tokens over up to 7 786 keys
+// 1.587e-3, with two halves and in 32 bits 1.586e-3; 3 989 prompt rows 1.574e-3 all three.  Two halves cost the prompts 491 -> 629 us, 27 rows over 8 274 keys 29.1 -> 32.8, single
+// tokens 47.0 -> 47.2.  fp32 rows, two halves of queries and weights: off by 4.6e-7 (prompts) and 4.9e-7 (two tokens) of the norm, products and sums of 24 bits by 8.6e-7 and 5.5e-7.
+//
 // Scales never touch an operand: a page's key scale multiplies its scores.  The second product takes w = e^(s - M) vscale, M the running maximum of s + ln vscale
 // over the keys a column has seen (so w <= 1 whatever the scales are, held as w 2^14 to keep halves normal down to 2^-28); the denominator sums e^(s - M) itself.
 //
@@ -12,8 +17,10 @@
 // neighbouring codes of a value column, one 16-byte load.  Pages have at least 16 tokens: a lane needs one page number and one pair of scales a step.
 //
 // Bound by the codes' bytes, which are read once, and before them by a chain of loads that each need the one before (tile, length, page number, keys: ~6 us of a launch).  Measured
-// (the launch alone; bf16, 4 heads a key head of 128): 64 single tokens over up to 8 192 keys, 189 MB, 37.7 us = 5.0 TB/s; one over 131 072, 268 MB, 44.4 us = 6.0 TB/s, 7.4 more its
-// merge; 27 rows over 8 247 keys of 32 heads, 68 MB, 25.5 us and 5.3: a wave has two steps of its own there.  A copy reaches 4.9 TB/s, a reading stream ~5.9.
+// (the launch alone, over caches that change from one to the next; bf16, 4 heads a key head of 128): 64 single tokens over up to 7 786 keys, 189 MB, 47.8 us = 4.0 TB/s; one over
+// 131 072, 268 MB, 54.3 us = 4.9 TB/s, 7.6 more its merge; 27 rows over 8 274 keys of 32 heads, 68 MB, 28.3 us and 5.9: a wave has two steps of its own there.  (The same cache again and
+// again, which the last-level cache holds in part: 37.7, 44.4 and 25.5.)  A copy reaches 4.9 TB/s, a reading stream ~5.9.  fp32 rows: the batch of tokens 49.5 us, the long one 63.7
+// with its merge, the 27 rows 58.
 #include "pb_attn_pages.h"
 
 namespace {

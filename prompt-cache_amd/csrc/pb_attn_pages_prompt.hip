@@ -6,8 +6,9 @@
 // first product's operand is key 16 (i / 2) + 8 h + 4 (i % 2) + j of 32, so lane half h holds keys 16 m + 8 h .. + 7), and a column's maximum is one exchange between two lanes.
 //
 // Bound by the two products and the softmax between them: a step of 64 keys is 2 x 16 MFMA and 32 exponentials a wave of heads of 128.  Measured: 3 989 rows of 32 heads of 128 over
-// 8 heads' prefixes of 4 096 .. 6 200 keys, bf16, 425 GFLOP: 480 us = 0.88 PFLOP/s, where a large fp16 product of the library reaches 1.12 (both lower the clock); fp32 (two halves
-// a number, so four times the products), 5 prompts of 1 877 rows of 15 heads of 96: 29 us, the 16 steps of the longest at 1.6 us each.
+// 8 heads' prefixes of 4 096 .. 6 200 keys, bf16, 425 GFLOP: 489 us = 0.87 PFLOP/s, where a large fp16 product of the library reaches 1.12 (both lower the clock); fp32 (two halves
+// of a query and of a weight under codes that are whole, so twice the products) 864 us.  5 prompts of 1 877 rows of 15 heads of 96 under a window of 333, fp32: 29 us, of which a block's
+// steps, at most 7, take 2.2 each and what is around them 15 (a window of 1: 17.3; in bf16 10.8): 230 workgroups of four waves, one a CU, have nothing beside a wave that waits.
 //
 // LDS rows are 16 bytes longer than their 32 ND halves of a key, or 64 keys of a value column: the sixteen lanes that are served at once fall on all banks.
 #include "pb_attn_pages.h"

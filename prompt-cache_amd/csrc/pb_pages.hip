@@ -2,12 +2,13 @@
 //
 // pcb_page_tables: every workgroup scans all sequences (a thread a sequence, in chunks of the workgroup) and knows each chunk's prefix sums; the flat rows,
 // tiles and pages of a chunk are then shared out among the workgroups, each found by a search in the chunk's sums in LDS.  A step's tables are bound by the
-// latency of the loads and of three scans one after the other, so a batch of one chunk and few rows is one workgroup.  Measured: 64 sequences of one token 6.7 us, 517 sequences
-// and 95 700 rows 11.0.
+// latency of the loads and of three scans one after the other, so a batch of one chunk and few rows is one workgroup.  Measured: 64 sequences of one token 6.6 us, 517 sequences
+// and 95 700 rows 11.0.  Where the new lengths take the old ones' place there is one workgroup for all rows: 64 sequences and 13 900 rows 22 us, 517 and 99 300 141 (8 apart).
 //
 // pcb_pages_append / pcb_pages_read: a wave takes the rows of one page (reading: 4 to 32 rows, of any pages) of one head, keys or values, by itself: no LDS, no barrier, and
 // the maximum of a page is a wave's reduction.  Both are bound by memory: rows in and codes out, each once.  Measured: 19 325 rows of 8 heads of 128 in and out again, 238 MB,
-// 58 us = 4.1 TB/s; 8 247 rows of 32 heads out, 203 MB, 32.5 us = 6.2 TB/s (a copy reaches 4.9: here twice as much is written as read).
+// 33.8 + 28.0 us = 3.8 TB/s; 8 247 rows of 32 heads out, 203 MB, 44.8 us = 4.5 TB/s (a copy reaches 4.9; into the same buffers again and again, which the last-level cache holds in
+// part, 32.5).
 #include "pb_pages.h"
 
 namespace {
