@@ -79,3 +79,17 @@ def test_far_scores_of_any_kind_stay_between_the_values(T, longest, dtype):
     bad[T, 3, 7] = float("nan")
     none = torch.isnan(r.run(T, q=bad, longest=longest))
     assert bool(none[T, 3].all()) and int(none.sum()) == 128
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("T, longest", FORMS)
+def test_far_scores_beside_a_sink(T, longest, dtype):
+    """One key a row, its score far above the sink or far below: its value, or 0."""
+    r = Requests([3000, 77], [T, T], 8, 2, 64, 32, "int8", dtype, seed=T + 3, scales=(24, 41))
+    r.q = torch.randn(r.q.shape, generator=torch.Generator(device=DEV).manual_seed(T), device=DEV).to(r.dtype)
+    got = r.run(T, window=1, longest=longest, sink=[2.5, -7.0, 0.0, 30.0] * 2)
+    z = O.attend(r.q.double().cpu().numpy(), r.seqs, r.pos, r.kv, r.table, r.kc, r.ks, r.vc, r.vs, r.P, r.kind, 1.0, 1, [2.5, -7.0, 0.0, 30.0] * 2)
+    alone = O.attend(r.q.double().cpu().numpy(), r.seqs, r.pos, r.kv, r.table, r.kc, r.ks, r.vc, r.vs, r.P, r.kind, 1.0, 1)
+    assert ((z == 0).all(-1) | (np.abs(z - alone) <= 2.0 ** -40 * np.abs(alone)).all(-1)).all()      # (so far are they: nothing in between)
+    assert 0 < (z == 0).all(-1).sum() < z[..., 0].size
+    assert (np.abs(got.double().cpu().numpy() - z) <= (torch.finfo(r.dtype).eps / 2 + 2.0 ** -21) * np.abs(z)).all()
